@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define OGMM_ABI_VERSION 28
+#define OGMM_ABI_VERSION 29
 
 int ogmm_abi_version(void);
 /* thread-local, valid until the next failing call on this thread */
@@ -525,6 +525,63 @@ int ogmm_pos_features(const float* xyz, const int32_t* idx, int C, int N, int k,
 
 /* ---- T7: backward of ogmm_l2norm_rows (models/gmmreg.py:74): dx = g/n - x (x.g)/n^3, n = max(|x|, 1e-12). */
 int ogmm_l2norm_rows_bwd(const float* x, int64_t ldx, const float* g, int64_t ldg, int64_t rows, int D, float* dx, int64_t lddx, void* stream);
+
+/* ---- L1-L3 (ABI 29): operators of large language models beside the path's own.  `type` codes of their tensors: */
+enum { OGMM_F32 = 0, OGMM_BF16 = 1, OGMM_F16 = 2 };
+
+/* ---- L1: attention of B x Nq query rows to Nk states of another sequence, H query heads over Hkv key / value heads (H % Hkv == 0; query head j reads key head
+ * j / (H / Hkv)), head width d (a multiple of 8 up to 128):
+ *     S = scale q k^T over the admitted keys,  P = softmax(S),  o = P v,  lse = log sum exp S.
+ * Admitted: key n < kv_lens[b] (NULL: Nk) and key_mask[b][n] != 0 (NULL: all); rows n >= q_lens[b] (NULL: Nq) and rows without an admitted key give o = 0, lse = -inf.
+ * Lengths outside [0, Nk] / [0, Nq] count as the nearer end.  What stands in keys and values that are not admitted, and in rows behind q_lens, does not matter
+ * (NaN and infinities among it).  Scores, statistics and sums are fp32; products of 16-bit types run on their matrix instructions (P and dS rounded to the type),
+ * those of fp32 on the fp32 ones.
+ * q, k, v, dout: element strides *_b (batch), *_n (row), *_h (head), channels contiguous; addresses and strides multiples of 16 bytes.  o, dq [B][Nq][H][d] and
+ * dk, dv [B][Nk][Hkv][d] contiguous, lse fp32 [B][H][Nq] (NULL in the forward: not wanted).  Every element of the outputs is written.  No atomics: repeated calls agree
+ * bit for bit.  workspace: ogmm_xattn_workspace_bytes(a, backward) bytes (0: NULL will do); it is used by this call alone. */
+typedef struct ogmm_xattn {
+    const void *q, *k, *v;
+    int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
+    void* o;
+    float* lse;
+    int32_t B, Nq, Nk, H, Hkv, d, type;
+    float scale;
+    const int32_t *q_lens, *kv_lens;
+    const uint8_t* key_mask;
+    int64_t mask_b;
+    /* backward: o and lse are inputs */
+    const void* dout;
+    int64_t do_b, do_n, do_h;
+    void *dq, *dk, *dv;
+    void* workspace;
+} ogmm_xattn;
+int64_t ogmm_xattn_workspace_bytes(const ogmm_xattn* a, int backward);
+int ogmm_xattn_fwd(const ogmm_xattn* a, void* stream);
+int ogmm_xattn_bwd(const ogmm_xattn* a, void* stream);
+
+/* ---- L2: root-mean-square norm of rows with the residual's addition: h = x + residual, rstd = 1 / sqrt(mean(h^2) + eps), y = h rstd w.  x, residual [rows][D] with row
+ * strides ldx, ldr; y, h [rows][D] contiguous of x's type (h: the stored sum, rounded; NULL without a residual), rstd fp32 [rows] or NULL.  weight [D]: x's type or fp32.  1 <= D <= 32768.
+ * _q8: y in 8 bits (e4m3, OCP) instead: scales s = max|y| / 448 over the row (group = 0; [rows]) or over each `group` = 32, 64, 128 columns ([rows][ceil(D / group)]), q = e4m3(y / s);
+ * s = q = 0 where max|y| / 448 is below 2^-126.
+ * _bwd: g = dy w, xh = h rstd: dx = rstd (g - xh mean(g xh)) + dh (dh = the stored sum's own gradient, NULL: none; dx is the residual's gradient too), dweight = sum over the rows
+ * of dy xh (weight's type); workspace: ogmm_rms_norm_bwd_workspace_bytes. */
+int ogmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int64_t rows, int D, int type, int weight_type, float eps,
+                  void* y, void* h, float* rstd, void* stream);
+int ogmm_rms_norm_q8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int64_t rows, int D, int type, int weight_type, float eps,
+                     int group, void* q, float* scales, void* h, void* stream);
+int64_t ogmm_rms_norm_bwd_workspace_bytes(int64_t rows, int D);
+int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight, const float* rstd, const void* dh, int64_t lddh, int64_t rows,
+                      int D, int type, int weight_type, void* dx, void* dweight, void* workspace, void* stream);
+
+/* ---- L3: global norm of n gradient tensors and their clipping: norm = inv_scale sqrt(sum of all squares), c = min(1, max_norm / (norm + 1e-6)), and every gradient times
+ * inv_scale c: in place (out = NULL) or into the fp32 tensors out[i].  grads, numel, types, out: HOST arrays of n entries (device pointers, element counts, type codes; read before the
+ * call returns); tensors may start at any element.  Squares are summed in fp64 in a fixed order.  A norm that is NaN makes the gradients NaN, an infinite one makes them 0 (NaN where they were
+ * infinite).  Written memory must not be shared between entries (refused); out[i] may be grads[i] itself where that is fp32.  norm: one fp32 on the device.
+ * workspace: ogmm_grad_norm_workspace_bytes(n, numel). */
+int64_t ogmm_grad_norm_workspace_bytes(int n, const int64_t* numel);
+int ogmm_grad_norm(int n, const void* const* grads, const int64_t* numel, const int32_t* types, float inv_scale, float* norm, void* workspace, void* stream);
+int ogmm_clip_grads(int n, const void* const* grads, const int64_t* numel, const int32_t* types, void* const* out, float inv_scale, float max_norm, float* norm,
+                    void* workspace, void* stream);
 
 /* ---- diagnostics (tools/edgeconv_time.py; not part of the hot path): OGMM_EDGECONV_PROBE=1 makes the fused EdgeConv kernels add the shader cycles of
  * their phases to a device counter, read and cleared here.  (The GEMM engines' ablation / clock-probe builds -- `precision` codes 12..40, 60..89,

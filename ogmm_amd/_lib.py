@@ -7,7 +7,7 @@ from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libogmm_hip.so")
 
-ABI_VERSION = 28
+ABI_VERSION = 29
 
 ACT_NONE, ACT_RELU, ACT_LEAKY02, ACT_SIGMOID = 0, 1, 2, 3
 PREC_F32, PREC_F16X3, PREC_F16X3_FRAG, PREC_F16_FRAG = 0, 1, 2, 3
@@ -40,6 +40,22 @@ class GemmDesc(Structure):
         ("terms", c_int32),
         ("nb_mean", c_void_p), ("nb_rstd", c_void_p), ("nb_scale", c_void_p), ("nb_shift", c_void_p), ("nb_act", c_int32),
         ("a_trans", c_int32), ("a_colsum", c_void_p),
+    ]
+
+
+class XattnDesc(Structure):
+    """Mirror of `struct ogmm_xattn`."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_b", c_int64), ("q_n", c_int64), ("q_h", c_int64), ("k_b", c_int64), ("k_n", c_int64), ("k_h", c_int64),
+        ("v_b", c_int64), ("v_n", c_int64), ("v_h", c_int64),
+        ("o", c_void_p), ("lse", c_void_p),
+        ("B", c_int32), ("Nq", c_int32), ("Nk", c_int32), ("H", c_int32), ("Hkv", c_int32), ("d", c_int32), ("type", c_int32),
+        ("scale", c_float),
+        ("q_lens", c_void_p), ("kv_lens", c_void_p), ("key_mask", c_void_p), ("mask_b", c_int64),
+        ("dout", c_void_p), ("do_b", c_int64), ("do_n", c_int64), ("do_h", c_int64),
+        ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+        ("workspace", c_void_p),
     ]
 
 
@@ -137,6 +153,16 @@ PROTOTYPES = {
     "ogmm_scatter_add_rows": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p],
     "ogmm_small_bmm_nt": [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p],
     "ogmm_l2norm_rows_bwd": [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p],
+    "ogmm_xattn_workspace_bytes": [POINTER(XattnDesc), c_int],
+    "ogmm_xattn_fwd": [POINTER(XattnDesc), c_void_p],
+    "ogmm_xattn_bwd": [POINTER(XattnDesc), c_void_p],
+    "ogmm_rms_norm": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
+    "ogmm_rms_norm_q8": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "ogmm_rms_norm_bwd_workspace_bytes": [c_int64, c_int],
+    "ogmm_rms_norm_bwd": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "ogmm_grad_norm_workspace_bytes": [c_int, c_void_p],
+    "ogmm_grad_norm": [c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p],
+    "ogmm_clip_grads": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float, c_void_p, c_void_p, c_void_p],
     "ogmm_debug_edgeconv_probe": [c_void_p],
     "ogmm_debug_edgeconv_pc_probe": [c_void_p],
     "ogmm_transpose_pad": [c_void_p, c_int64, c_int64, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p],

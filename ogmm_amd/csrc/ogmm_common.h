@@ -48,6 +48,12 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 
+// fp32 -> the bits of a 16-bit type (OGMM_BF16 / OGMM_F16), round to nearest even
+__device__ __forceinline__ uint16_t to_half_bits(float x, int type) {
+    if (type == OGMM_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
+}
+
 // exact-rounding fp32 primitives: the compiler must not contract these (discrete choices depend on them)
 __device__ __forceinline__ float mul_rn(float a, float b) { return __fmul_rn(a, b); }
 __device__ __forceinline__ float add_rn(float a, float b) { return __fadd_rn(a, b); }

@@ -1,0 +1,379 @@
+// Root-mean-square norm of rows with the residual's addition:
+//     h = x + r,   rstd = 1 / sqrt(mean(h^2) + eps),   y = h rstd w          (one pass: the row stays in registers between its sum and its output)
+// its gradient, with g = dy w and xh = h rstd,
+//     dx = rstd (g - xh mean(g xh)) + dh,   dw = sum over rows of dy xh,
+// and its output in 8 bits: s = max|y| / 448 over the row or over each group of its columns, q = e4m3(y / s).
+//
+// Bound by HBM: a few operations for each value read or written.  A row is taken by 8, 64, 256 or 1024 lanes, so that a lane holds at most 32 values of it (one to
+// eight loads of sixteen bytes, all in flight before the first is used) and the sum is one exchange inside a wave, or one through LDS.  The weights of a lane's
+// columns are read once and stay in registers for all the rows that its workgroup takes.  Rows may start anywhere (odd widths, strides): the part reads sixteen
+// bytes from any address; only a row's last, partial piece goes value by value.
+#include "ogmm_common.h"
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+using namespace ogmm;
+
+constexpr int MAX_D = 32768;
+constexpr float E4M3_MAX = 448.0f;
+
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[N]; };
+template <int N>
+struct __attribute__((packed, aligned(1))) Bytes { uint32_t w[N / 4]; };
+
+// values [c, c + N) of a row of D; zeros behind its end
+template <int N, class T>
+__device__ __forceinline__ void load(const T* __restrict__ row, int c, int D, float (&out)[N]) {
+    if (c + N <= D) {
+        const Piece<T, N> p = *reinterpret_cast<const Piece<T, N>*>(row + c);
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = static_cast<float>(p.v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = c + k < D ? static_cast<float>(row[c + k]) : 0.0f;
+    }
+}
+
+template <int N, class T>
+__device__ __forceinline__ void store(T* __restrict__ row, int c, int D, const float (&x)[N]) {
+    if (c + N <= D) {
+        Piece<T, N> p;
+#pragma unroll
+        for (int k = 0; k < N; ++k) p.v[k] = static_cast<T>(x[k]);
+        *reinterpret_cast<Piece<T, N>*>(row + c) = p;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (c + k < D) row[c + k] = static_cast<T>(x[k]);
+    }
+}
+
+// Sum (or maximum) over the LANES lanes of one row; every lane gets it.  `slot` alternates between rows, so that one barrier a row is enough.
+template <int LANES, bool MAX>
+__device__ __forceinline__ float over_row(float v, float* lds, int& slot) {
+#pragma unroll
+    for (int o = 1; o < (LANES < 64 ? LANES : 64); o <<= 1) {
+        const float u = __shfl_xor(v, o, 64);
+        v = MAX ? fmaxf(v, u) : v + u;
+    }
+    if constexpr (LANES > 64) {
+        constexpr int W = LANES / 64;
+        float* s = lds + slot * W;
+        slot ^= 1;
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = s[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) v = MAX ? fmaxf(v, s[i]) : v + s[i];
+    }
+    return v;
+}
+
+template <int LANES> constexpr int THREADS = LANES > 256 ? LANES : 256;
+
+struct NormArgs {
+    const void *x, *r, *w;
+    int64_t ldx, ldr, rows;
+    int D, group;
+    float eps;
+    void *y, *h;
+    float *rstd, *scales;
+};
+
+// Q8: y in 8 bits with scales
+template <class T, class W, int LANES, int ITEMS, bool Q8>
+__global__ __launch_bounds__(THREADS<LANES>) void rms_norm_kernel(const NormArgs a) {
+    constexpr int VEC = 16 / sizeof(T), PER = THREADS<LANES> / LANES;
+    __shared__ float lds[2 * (LANES > 64 ? LANES / 64 : 1)];
+    int slot = 0;
+    const int lane = threadIdx.x % LANES, D = a.D;
+    float w[ITEMS][VEC];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) load<VEC>(static_cast<const W*>(a.w), (i * LANES + lane) * VEC, D, w[i]);
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * PER; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * PER) {
+        const int64_t row = row0 + threadIdx.x / LANES;
+        const bool here = LANES > 64 || row < a.rows;          // (a row's lanes agree; lanes of one wave may hold several rows and take part in the exchange)
+        const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+        float h[ITEMS][VEC];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) load<VEC>(x, (i * LANES + lane) * VEC, here ? D : 0, h[i]);
+        if (a.r) {
+            const T* r = static_cast<const T*>(a.r) + row * a.ldr;
+            float u[ITEMS][VEC];
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) load<VEC>(r, (i * LANES + lane) * VEC, here ? D : 0, u[i]);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) h[i][k] += u[i][k];
+                // (the stored sum is rounded to the type of the stream it belongs to; the norm below takes the sum itself)
+                store<VEC>(static_cast<T*>(a.h) + row * D, (i * LANES + lane) * VEC, here ? D : 0, h[i]);
+            }
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) ss = fmaf(h[i][k], h[i][k], ss);
+        ss = over_row<LANES, false>(ss, lds, slot);
+        const float rstd = 1.0f / sqrtf(ss / D + a.eps);
+        if constexpr (!Q8) {
+            if (a.rstd && here && lane == 0) a.rstd[row] = rstd;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * rstd * w[i][k];
+                store<VEC>(static_cast<T*>(a.y) + row * D, (i * LANES + lane) * VEC, here ? D : 0, h[i]);
+            }
+        } else {
+            // rstd > 0 leaves y / s as it is where both lack it: t = h w, s = rstd max|t| / 448, q = e4m3(t 448 / max|t|), one rounding less than through y
+            const int groups = a.group ? (D + a.group - 1) / a.group : 1;
+            float top[ITEMS];
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                top[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    h[i][k] *= w[i][k];
+                    top[i] = fmaxf(top[i], fabsf(h[i][k]));
+                }
+            }
+            if (a.group) {
+                for (int o = 1; o < a.group / VEC; o <<= 1)          // (a group's lanes are neighbours in one wave: 32, 64 or 128 columns)
+#pragma unroll
+                    for (int i = 0; i < ITEMS; ++i) top[i] = fmaxf(top[i], __shfl_xor(top[i], o, 64));
+            } else {
+                float m = top[0];
+#pragma unroll
+                for (int i = 1; i < ITEMS; ++i) m = fmaxf(m, top[i]);
+                m = over_row<LANES, true>(m, lds, slot);
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) top[i] = m;
+            }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c = (i * LANES + lane) * VEC;
+                float s = top[i] * rstd / E4M3_MAX;
+                if (s < 1.17549435e-38f) s = 0.0f;          // (below the normal numbers the quotient y / s would not be defined to 4 bits)
+                const float up = top[i] < 1e-30f ? 0x1p100f : 1.0f;          // 448 / max|t| stays finite
+                const float inv = s == 0.0f ? 0.0f : E4M3_MAX / (top[i] * up);
+                if (here && c < D && (a.group ? c % a.group == 0 : c == 0)) a.scales[row * groups + (a.group ? c / a.group : 0)] = s;
+                float q[VEC];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) q[k] = h[i][k] * up * inv;
+                Bytes<VEC> b;
+#pragma unroll
+                for (int k = 0; k < VEC; k += 4)
+                    b.w[k / 4] = (__builtin_amdgcn_cvt_pk_fp8_f32(q[k], q[k + 1], 0, false) & 0xffff) | __builtin_amdgcn_cvt_pk_fp8_f32(q[k + 2], q[k + 3], 0, false) << 16;
+                uint8_t* o = static_cast<uint8_t*>(a.y) + row * D + c;
+                if (here && c + VEC <= D) *reinterpret_cast<Bytes<VEC>*>(o) = b;
+                else
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k)
+                        if (here && c + k < D) o[k] = static_cast<uint8_t>(b.w[k / 4] >> (k % 4 * 8));
+            }
+        }
+    }
+}
+
+struct BwdArgs {
+    const void *dy, *h, *w, *dh;
+    const float* rstd;
+    int64_t lddy, ldh, lddh, rows;
+    int D;
+    void* dx;
+    float* part;          // [gridDim.x][D]: each workgroup's share of dw
+};
+
+template <class T, class W, int LANES, int ITEMS>
+__global__ __launch_bounds__(THREADS<LANES>) void rms_norm_bwd_kernel(const BwdArgs a) {
+    constexpr int VEC = 16 / sizeof(T), PER = THREADS<LANES> / LANES;
+    __shared__ float lds[2 * (LANES > 64 ? LANES / 64 : 1)];
+    __shared__ float share[PER > 1 ? PER * LANES * VEC : 1];
+    int slot = 0;
+    const int lane = threadIdx.x % LANES, D = a.D;
+    float w[ITEMS][VEC], dw[ITEMS][VEC];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        load<VEC>(static_cast<const W*>(a.w), (i * LANES + lane) * VEC, D, w[i]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dw[i][k] = 0.0f;
+    }
+    const float inv_d = 1.0f / D;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * PER; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * PER) {
+        const int64_t row = row0 + threadIdx.x / LANES;
+        const bool here = LANES > 64 || row < a.rows;
+        const int d = here ? D : 0;
+        const T *dy = static_cast<const T*>(a.dy) + row * a.lddy, *h = static_cast<const T*>(a.h) + row * a.ldh;
+        const float rstd = here ? a.rstd[row] : 0.0f;
+        float g[ITEMS][VEC], xh[ITEMS][VEC];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            load<VEC>(dy, (i * LANES + lane) * VEC, d, g[i]);
+            load<VEC>(h, (i * LANES + lane) * VEC, d, xh[i]);
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                xh[i][k] *= rstd;
+                dw[i][k] = fmaf(g[i][k], xh[i][k], dw[i][k]);
+                g[i][k] *= w[i][k];
+                dot = fmaf(g[i][k], xh[i][k], dot);
+            }
+        dot = over_row<LANES, false>(dot, lds, slot) * inv_d;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            float dx[VEC];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) dx[k] = rstd * (g[i][k] - xh[i][k] * dot);
+            if (a.dh) {
+                float u[VEC];
+                load<VEC>(static_cast<const T*>(a.dh) + row * a.lddh, (i * LANES + lane) * VEC, d, u);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) dx[k] += u[k];
+            }
+            store<VEC>(static_cast<T*>(a.dx) + row * D, (i * LANES + lane) * VEC, d, dx);
+        }
+    }
+    float* part = a.part + static_cast<int64_t>(blockIdx.x) * D;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        if constexpr (PER == 1) {
+            store<VEC>(part, (i * LANES + lane) * VEC, D, dw[i]);
+        } else {          // the workgroup's rows side by side: one sum over them, in their order
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) share[threadIdx.x * VEC + k] = dw[i][k];
+            __syncthreads();
+            for (int e = threadIdx.x; e < LANES * VEC; e += THREADS<LANES>) {
+                float s = 0.0f;
+                for (int p = 0; p < PER; ++p) s += share[p * LANES * VEC + e];
+                const int c = i * LANES * VEC + e;
+                if (c < D) part[c] = s;
+            }
+        }
+    }
+}
+
+// dw[c] = sum over the workgroups' shares: 64 columns to a workgroup, sixteen slices of the shares beside each other
+template <class W>
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restrict__ part, int n, int D, W* __restrict__ dw) {
+    __shared__ double lds[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), s = threadIdx.x >> 6;
+    double acc = 0.0;
+    if (c < D)
+#pragma unroll 8
+        for (int i = s; i < n; i += 16) acc += part[static_cast<int64_t>(i) * D + c];
+    lds[s][threadIdx.x & 63] = acc;
+    __syncthreads();
+    if (s == 0 && c < D) {
+        for (int i = 1; i < 16; ++i) acc += lds[i][threadIdx.x];
+        dw[c] = static_cast<W>(static_cast<float>(acc));
+    }
+}
+
+// Lanes to a row and loads of sixteen bytes to a lane: the fewest lanes that keep a lane at four loads (narrow rows: two), so that narrow rows share a workgroup
+template <class T, class F>
+int with_shape(int D, int least_lanes, F&& f) {
+    constexpr int VEC = 16 / sizeof(T);
+    using std::integral_constant;
+    auto go = [&](auto lanes, auto items) { return f(lanes, items); };
+    const int n = (D + VEC - 1) / VEC;
+#define OGMM_SHAPE(L, I) if (n <= L * I && least_lanes <= L) return go(integral_constant<int, L>(), integral_constant<int, I>())
+    OGMM_SHAPE(8, 1);
+    OGMM_SHAPE(8, 2);
+    OGMM_SHAPE(64, 1);
+    OGMM_SHAPE(64, 2);
+    OGMM_SHAPE(64, 4);
+    OGMM_SHAPE(256, 2);
+    OGMM_SHAPE(256, 4);
+    OGMM_SHAPE(1024, 2);
+    OGMM_SHAPE(1024, 4);
+    if constexpr (sizeof(T) == 4) OGMM_SHAPE(1024, 8);
+#undef OGMM_SHAPE
+    return fail("rms_norm: rows of %d values are too wide", D);
+}
+
+// workgroups: as many as the rows need, and no more than fill the 256 CUs a few times over (each reads the weights once)
+inline int blocks_for(int64_t rows, int per, int most) { return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, most)); }
+
+template <class T, class W>
+int launch_norm(const NormArgs& a, bool q8, hipStream_t stream) {
+    return with_shape<T>(a.D, a.group ? 64 : 1, [&](auto lanes, auto items) {
+        constexpr int L = decltype(lanes)::value, I = decltype(items)::value;
+        const int blocks = blocks_for(a.rows, THREADS<L> / L, L > 256 ? 1024 : 4096);
+        if (q8) rms_norm_kernel<T, W, L, I, true><<<blocks, THREADS<L>, 0, stream>>>(a);
+        else rms_norm_kernel<T, W, L, I, false><<<blocks, THREADS<L>, 0, stream>>>(a);
+        return check_launch("ogmm_rms_norm");
+    });
+}
+
+constexpr int BWD_BLOCKS = 512;
+
+template <class T, class W>
+int launch_bwd(const BwdArgs& a, void* dw, hipStream_t stream) {
+    return with_shape<T>(a.D, 1, [&](auto lanes, auto items) {
+        constexpr int L = decltype(lanes)::value, I = decltype(items)::value;
+        const int blocks = blocks_for(a.rows, THREADS<L> / L, BWD_BLOCKS);
+        if (blocks) rms_norm_bwd_kernel<T, W, L, I><<<blocks, THREADS<L>, 0, stream>>>(a);
+        rms_norm_dw_kernel<W><<<(a.D + 63) / 64, 1024, 0, stream>>>(a.part, blocks, a.D, static_cast<W*>(dw));
+        return check_launch("ogmm_rms_norm_bwd");
+    });
+}
+
+template <class F>
+int with_types(const char* who, int type, int wtype, F&& f) {
+    if (type == OGMM_F32 && wtype == OGMM_F32) return f(float(), float());
+    if (type == OGMM_BF16 && wtype == OGMM_BF16) return f(__bf16(), __bf16());
+    if (type == OGMM_BF16 && wtype == OGMM_F32) return f(__bf16(), float());
+    if (type == OGMM_F16 && wtype == OGMM_F16) return f(_Float16(), _Float16());
+    if (type == OGMM_F16 && wtype == OGMM_F32) return f(_Float16(), float());
+    return fail("%s: rows of type %d with weights of type %d are not supported", who, type, wtype);
+}
+
+int check_rows(const char* who, int64_t rows, int D) {
+    OGMM_REQUIRE(rows >= 0, "%s: negative number of rows", who);
+    OGMM_REQUIRE(D >= 1 && D <= MAX_D, "%s: rows of %d values (1 to %d are supported)", who, D, MAX_D);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int ogmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int64_t rows, int D, int type, int weight_type, float eps,
+                             void* y, void* h, float* rstd, void* stream) {
+    if (check_rows("ogmm_rms_norm", rows, D)) return 1;
+    OGMM_REQUIRE(weight && (!rows || (x && y)) && (!rows || !residual || h), "ogmm_rms_norm: missing argument");
+    OGMM_REQUIRE(eps >= 0.0f, "ogmm_rms_norm: eps must not be negative");
+    if (!rows) return 0;
+    const NormArgs a{x, residual, weight, ldx, ldr, rows, D, 0, eps, y, h, rstd, nullptr};
+    return with_types("ogmm_rms_norm", type, weight_type, [&](auto t, auto w) { return launch_norm<decltype(t), decltype(w)>(a, false, as_stream(stream)); });
+}
+
+extern "C" int ogmm_rms_norm_q8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int64_t rows, int D, int type, int weight_type, float eps,
+                                int group, void* q, float* scales, void* h, void* stream) {
+    if (check_rows("ogmm_rms_norm_q8", rows, D)) return 1;
+    OGMM_REQUIRE(weight && (!rows || (x && q && scales)) && (!rows || !residual || h), "ogmm_rms_norm_q8: missing argument");
+    OGMM_REQUIRE(eps >= 0.0f, "ogmm_rms_norm_q8: eps must not be negative");
+    OGMM_REQUIRE(group == 0 || group == 32 || group == 64 || group == 128, "ogmm_rms_norm_q8: group must be 0 (the row), 32, 64 or 128 columns, got %d", group);
+    if (!rows) return 0;
+    const NormArgs a{x, residual, weight, ldx, ldr, rows, D, group, eps, q, h, nullptr, scales};
+    return with_types("ogmm_rms_norm_q8", type, weight_type, [&](auto t, auto w) { return launch_norm<decltype(t), decltype(w)>(a, true, as_stream(stream)); });
+}
+
+extern "C" int64_t ogmm_rms_norm_bwd_workspace_bytes(int64_t rows, int D) {
+    if (rows < 0 || D < 1) return -1;
+    return std::max<int64_t>(1, std::min<int64_t>(rows, BWD_BLOCKS)) * D * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight, const float* rstd, const void* dh, int64_t lddh, int64_t rows,
+                                 int D, int type, int weight_type, void* dx, void* dweight, void* workspace, void* stream) {
+    if (check_rows("ogmm_rms_norm_bwd", rows, D)) return 1;
+    OGMM_REQUIRE(weight && dweight && workspace && (!rows || (dy && h && rstd && dx)), "ogmm_rms_norm_bwd: missing argument");
+    const BwdArgs a{dy, h, weight, dh, rstd, lddy, ldh, lddh, rows, D, dx, static_cast<float*>(workspace)};
+    return with_types("ogmm_rms_norm_bwd", type, weight_type, [&](auto t, auto w) { return launch_bwd<decltype(t), decltype(w)>(a, dweight, as_stream(stream)); });
+}

@@ -1166,3 +1166,262 @@ def weight_grad_thin(dy, x, split=False, overflow=None):
     else:
         _lib.call("ogmm_weight_grad_thin", _p(_f32(dy, "dy")), dy.stride(0), _p(_f32(x, "x")), x.stride(0), R, n, k, _p(part), _stream())
     return part.sum(dim=0)
+
+
+# ---------------------------------------------------------------------------------------------- operators of large language models (csrc/cross_attention.hip, rms_norm.hip, train_clip.hip)
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # OGMM_F32 / OGMM_BF16 / OGMM_F16
+
+
+def _dev(name, first, *others):
+    """The device of a call's tensors: all on one GPU, of a type that has kernels; others: (name, tensor or None)."""
+    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+        raise _lib.OgmmError("%s must be a CUDA/ROCm tensor (the HIP path has no CPU fallback)" % name)
+    for n, t in others:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.device != first.device):
+            raise _lib.OgmmError("%s must be a tensor on %s" % (n, first.device))
+    return first.device
+
+
+def _code(t, name):
+    c = _TYPE.get(t.dtype)
+    if c is None:
+        raise _lib.OgmmError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return c
+
+
+def _call_on(dev, name, *args):
+    """_lib.call on the tensors' own device and on torch's current stream OF that device, whichever device is current (the stream comes last)."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        return
+    with torch.cuda.device(dev):
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _heads(t, name, like=None):
+    """[B, n, heads, d] as the attention kernels take it: channels contiguous, address and strides multiples of 16 bytes (anything else is copied)"""
+    if t.dim() != 4:
+        raise _lib.OgmmError("%s must be [B, n, heads, d], got %s" % (name, tuple(t.shape)))
+    if like is not None and t.dtype != like.dtype:
+        raise _lib.OgmmError("%s must be %s, got %s" % (name, like.dtype, t.dtype))
+    b, n, h, one = t.stride()
+    step = 16 // t.element_size()
+    if (one != 1 and t.shape[3] != 1) or (b | n | h) % step or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:          # (contiguous already, at an odd address)
+            t = t.clone()
+    return t
+
+
+def _lens(t, B, name):
+    if t is None:
+        return None
+    if _i32(t, name).shape != (B,):
+        raise _lib.OgmmError("%s must have one entry for each of the %d batch entries, got %s" % (name, B, tuple(t.shape)))
+    return t.contiguous()
+
+
+def _xattn(q, k, v, kv_lens, q_lens, key_mask, scale):
+    dev = _dev("q", q, ("k", k), ("v", v), ("kv_lens", kv_lens), ("q_lens", q_lens), ("key_mask", key_mask))
+    code = _code(q, "q")
+    q, k, v = _heads(q, "q"), _heads(k, "k", q), _heads(v, "v", q)
+    B, Nq, H, d = q.shape
+    Nk, Hkv = k.shape[1:3]
+    if k.shape != (B, Nk, Hkv, d) or v.shape != k.shape:
+        raise _lib.OgmmError("q %s, k %s and v %s do not fit: [B, Nq, H, d] and twice [B, Nk, Hkv, d]" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    kv_lens, q_lens = _lens(kv_lens, B, "kv_lens"), _lens(q_lens, B, "q_lens")
+    if key_mask is not None:
+        if key_mask.shape != (B, Nk) or key_mask.dtype != torch.bool:
+            raise _lib.OgmmError("key_mask must be bool [%d, %d], got %s %s" % (B, Nk, key_mask.dtype, tuple(key_mask.shape)))
+        if key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+    a = _lib.XattnDesc()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_b, a.q_n, a.q_h, _ = q.stride()
+    a.k_b, a.k_n, a.k_h, _ = k.stride()
+    a.v_b, a.v_n, a.v_h, _ = v.stride()
+    a.B, a.Nq, a.Nk, a.H, a.Hkv, a.d, a.type = B, Nq, Nk, H, Hkv, d, code
+    a.scale = d ** -0.5 if scale is None else scale
+    a.q_lens = None if q_lens is None else q_lens.data_ptr()
+    a.kv_lens = None if kv_lens is None else kv_lens.data_ptr()
+    if key_mask is not None:
+        a.key_mask, a.mask_b = key_mask.data_ptr(), key_mask.stride(0)
+    return a, dev, (q, k, v, kv_lens, q_lens, key_mask)          # (the tensors: alive until the kernels are enqueued)
+
+
+def _xattn_call(name, a, dev, backward):
+    nbytes = _lib.load().ogmm_xattn_workspace_bytes(ctypes.byref(a), backward)
+    ws = None
+    if nbytes > 0:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        a.workspace = ws.data_ptr()
+    _call_on(dev, name, ctypes.byref(a))
+
+
+def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=None, need_lse=False):
+    """Attention of query rows to states of another sequence: softmax(scale q k^T) v over each row's admitted keys.
+    q [B, Nq, H, d]; k, v [B, Nk, Hkv, d], H a multiple of Hkv (query head j reads key head j // (H // Hkv)); d a multiple of 8 up to 128; float32, bfloat16 or
+    float16, any strides (channels contiguous and 16-byte steps are taken as they are, anything else is copied).  kv_lens / q_lens int32 [B]: how many of the
+    padded keys / rows are there; key_mask bool [B, Nk]: True = admitted.  scale: default d ** -0.5.  A row without an admitted key, or behind q_lens, gives zeros;
+    what stands in keys that are not admitted does not matter.  -> o [B, Nq, H, d], with need_lse also log sum exp of the scores, fp32 [B, H, Nq] (-inf for such rows).
+    One row or a few against many keys are split over the keys.  For attention to at most 128 anchors of equal clouds see attention()."""
+    a, dev, held = _xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
+    o = torch.empty(held[0].shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((a.B, a.H, a.Nq), dtype=torch.float32, device=dev) if need_lse else None
+    a.o, a.lse = o.data_ptr(), None if lse is None else lse.data_ptr()
+    _xattn_call("ogmm_xattn_fwd", a, dev, 0)
+    return (o, lse) if need_lse else o
+
+
+def cross_attention_bwd(q, k, v, o, lse, dout, kv_lens=None, q_lens=None, key_mask=None, scale=None):
+    """Backward of cross_attention(): (dq, dk, dv) from dout = dL/do and the forward's o and lse; the scores are formed again.  Gradients of a key head are summed over
+    the query heads that share it; keys that are not admitted and rows behind q_lens get zeros.  Repeated calls agree bit for bit."""
+    a, dev, held = _xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
+    _dev("q", held[0], ("o", o), ("lse", lse), ("dout", dout))
+    if o.shape != held[0].shape or dout.shape != held[0].shape or lse.shape != (a.B, a.H, a.Nq):
+        raise _lib.OgmmError("o %s, dout %s and lse %s must be shaped as cross_attention() returns them for q %s" % (tuple(o.shape), tuple(dout.shape), tuple(lse.shape), tuple(q.shape)))
+    if o.dtype != q.dtype:
+        raise _lib.OgmmError("o must be %s, got %s" % (q.dtype, o.dtype))
+    dout, o, lse = _heads(dout, "dout", q), _heads(o.contiguous(), "o"), _f32(lse, "lse").contiguous()
+    dq = torch.empty(held[0].shape, dtype=q.dtype, device=dev)
+    dk, dv = (torch.empty(held[1].shape, dtype=q.dtype, device=dev) for _ in range(2))
+    a.o, a.lse, a.dout = o.data_ptr(), lse.data_ptr(), dout.data_ptr()
+    a.do_b, a.do_n, a.do_h, _ = dout.stride()
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    _xattn_call("ogmm_xattn_bwd", a, dev, 1)
+    return dq, dk, dv
+
+
+def _rows(t, D, name):
+    """[..., D] as rows with contiguous values -> (2-D view or copy, row stride)"""
+    t = t.reshape(-1, D)
+    if t.stride(1) != 1 and D != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _norm_args(x, weight, residual):
+    dev = _dev("x", x, ("weight", weight), ("residual", residual))
+    code = _code(x, "x")
+    if x.dim() < 1 or not x.shape[-1] or weight.shape != x.shape[-1:]:
+        raise _lib.OgmmError("weight must have one value for each of the last axis of x %s, got %s" % (tuple(x.shape), tuple(weight.shape)))
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        raise _lib.OgmmError("weight must be %s or float32, got %s" % (x.dtype, weight.dtype))
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise _lib.OgmmError("residual must be %s %s, got %s %s" % (x.dtype, tuple(x.shape), residual.dtype, tuple(residual.shape)))
+    return dev, code, weight.contiguous()
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight over the last axis (up to 32768 values).  x [..., D] float32, bfloat16 or float16 (rows with any stride);
+    weight [D] of x's type or float32.  -> (y, h, rstd): h = x itself without a residual, otherwise the sum rounded to x's type (y is formed from the sum before
+    that rounding); rstd fp32, one value a row, is what rms_norm_bwd() takes."""
+    dev, code, w = _norm_args(x, weight, residual)
+    D = x.shape[-1]
+    x2, ldx = _rows(x, D, "x")
+    r2, ldr = _rows(residual, D, "residual") if residual is not None else (None, 0)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    _call_on(dev, "ogmm_rms_norm", x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps,
+             y.data_ptr(), None if residual is None else h.data_ptr(), rstd.data_ptr())
+    return y, h, rstd
+
+
+def rms_norm_q8(x, weight, residual=None, eps=1e-6, group=0):
+    """rms_norm() with y in 8 bits: -> (q float8_e4m3fn [..., D], scales fp32, h); y = q * scale.  One scale a row (group = 0: scales [..., 1]) or one for each `group` = 32, 64 or
+    128 columns (scales [..., ceil(D / group)]), the largest magnitude over 448."""
+    dev, code, w = _norm_args(x, weight, residual)
+    if group not in (0, 32, 64, 128):
+        raise _lib.OgmmError("group must be 0 (one scale a row), 32, 64 or 128 columns, got %r" % (group,))
+    D = x.shape[-1]
+    x2, ldx = _rows(x, D, "x")
+    r2, ldr = _rows(residual, D, "residual") if residual is not None else (None, 0)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scales = torch.empty(x.shape[:-1] + (-(-D // group) if group else 1,), dtype=torch.float32, device=dev)
+    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    _call_on(dev, "ogmm_rms_norm_q8", x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps, group,
+             q.data_ptr(), scales.data_ptr(), None if residual is None else h.data_ptr())
+    return q, scales, h
+
+
+def rms_norm_bwd(dy, h, weight, rstd, dh=None):
+    """Backward of rms_norm(): (dx, dweight) from dy = dL/dy, the forward's h and rstd, and dh = dL/dh where the sum has readers of its own; dx is the residual's gradient too."""
+    dev, code, w = _norm_args(h, weight, None)
+    _dev("h", h, ("dy", dy), ("rstd", rstd), ("dh", dh))
+    for n, t in (("dy", dy), ("dh", dh)):
+        if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
+            raise _lib.OgmmError("%s must be %s %s, got %s %s" % (n, h.dtype, tuple(h.shape), t.dtype, tuple(t.shape)))
+    if _f32(rstd, "rstd").shape != h.shape[:-1]:
+        raise _lib.OgmmError("rstd must have one value for each row of h %s, got %s" % (tuple(h.shape), tuple(rstd.shape)))
+    D = h.shape[-1]
+    (dy2, lddy), (h2, ldh), rstd = _rows(dy, D, "dy"), _rows(h, D, "h"), rstd.contiguous()
+    dh2, lddh = _rows(dh, D, "dh") if dh is not None else (None, 0)
+    dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    dw = torch.empty(D, dtype=w.dtype, device=dev)
+    ws = torch.empty(_lib.load().ogmm_rms_norm_bwd_workspace_bytes(h2.shape[0], D), dtype=torch.uint8, device=dev)
+    _call_on(dev, "ogmm_rms_norm_bwd", dy2.data_ptr(), lddy, h2.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), None if dh2 is None else dh2.data_ptr(), lddh, h2.shape[0], D,
+             code, _TYPE[w.dtype], dx.data_ptr(), dw.data_ptr(), ws.data_ptr())
+    return dx, dw
+
+
+def _dense(t):
+    """True where a tensor's elements fill one stretch of memory without gaps or overlaps, in any order of its axes"""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s != 1), key=lambda p: p[1]):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _grad_list(grads, name="gradient"):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise _lib.OgmmError("no %s tensors given" % name)
+    dev = _dev("%s 0" % name, grads[0])
+    n = len(grads)
+    types = []
+    for i, g in enumerate(grads):
+        c = _TYPE.get(g.dtype) if isinstance(g, torch.Tensor) and g.layout is torch.strided else None
+        if c is None or g.device != dev:
+            raise _lib.OgmmError("%s %d must be a dense float32, bfloat16 or float16 tensor on %s" % (name, i, dev))
+        if not _dense(g):
+            raise _lib.OgmmError("%s %d has gaps or overlaps between its elements (shape %s, strides %s)" % (name, i, tuple(g.shape), g.stride()))
+        types.append(c)
+    return grads, dev, n, (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]), (ctypes.c_int32 * n)(*types)
+
+
+def grad_norm(grads, inv_scale=1.0):
+    """inv_scale * sqrt(sum of the squares of all values of all tensors): fp32 scalar on the device.  grads: float32, bfloat16 and float16 tensors, mixed as they come."""
+    grads, dev, n, ptrs, numel, types = _grad_list(grads)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(_lib.load().ogmm_grad_norm_workspace_bytes(n, numel), dtype=torch.uint8, device=dev)
+    _call_on(dev, "ogmm_grad_norm", n, ptrs, numel, types, inv_scale, norm.data_ptr(), ws.data_ptr())
+    return norm
+
+
+def clip_grads_(grads, max_norm, inv_scale=1.0, out=None):
+    """Scales the tensors by inv_scale * min(1, max_norm / (norm + 1e-6)) with norm = grad_norm(grads, inv_scale), in place, or into the fp32 tensors `out` (same shapes; the
+    gradients stay as they are).  inv_scale: the inverse of the loss scale that the gradients carry.  max_norm may be infinite (un-scale only).  -> norm, fp32 scalar on the device; no host
+    synchronisation.  A NaN norm makes every gradient NaN.  Tensors that share memory which is written are refused."""
+    grads, dev, n, ptrs, numel, types = _grad_list(grads)
+    outs = None
+    if out is not None:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != n:
+            raise _lib.OgmmError("out must hold a tensor for each of the %d gradients, got %d" % (n, len(out)))
+        for i, (g, o) in enumerate(zip(grads, out)):
+            if not isinstance(o, torch.Tensor) or o.device != dev or o.dtype != torch.float32 or o.shape != g.shape:
+                raise _lib.OgmmError("out %d must be a float32 tensor %s on %s" % (i, tuple(g.shape), dev))
+            if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                raise _lib.OgmmError("out %d must have the strides of its gradient" % i)
+            if not _dense(o):
+                raise _lib.OgmmError("out %d has gaps or overlaps between its elements (shape %s, strides %s)" % (i, tuple(o.shape), o.stride()))
+        outs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(_lib.load().ogmm_grad_norm_workspace_bytes(n, numel), dtype=torch.uint8, device=dev)
+    _call_on(dev, "ogmm_clip_grads", n, ptrs, numel, types, outs, inv_scale, max_norm, norm.data_ptr(), ws.data_ptr())
+    return norm

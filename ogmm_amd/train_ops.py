@@ -790,3 +790,53 @@ class TrainOps:
     def rotation_from_cov(self, M):
         """baseline/deepgmr.py:28-34: M [B,3,3] -> R [B,3,3], differentiable"""
         return _RotationFromCov.apply(M.contiguous())
+
+
+# ---------------------------------------------------------------------------------------------- operators of large language models, differentiable
+class _CrossAttention(torch.autograd.Function):
+    """ops.cross_attention with its gradient; saves o and the rows' log sum exp, never the scores"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens, q_lens, key_mask, scale):
+        o, lse = ops.cross_attention(q, k, v, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask, scale=scale, need_lse=True)
+        ctx.save_for_backward(q, k, v, o, lse, kv_lens, q_lens, key_mask)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, o, lse, kv_lens, q_lens, key_mask = ctx.saved_tensors
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, g, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask, scale=ctx.scale)
+        return dq, dk, dv, None, None, None, None
+
+
+def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=None):
+    """ops.cross_attention(q, k, v, ...) with autograd: q [B, Nq, H, d], k, v [B, Nk, Hkv, d] -> [B, Nq, H, d]"""
+    return _CrossAttention.apply(q, k, v, kv_lens, q_lens, key_mask, scale)
+
+
+class _RmsNorm(torch.autograd.Function):
+    """ops.rms_norm with its gradient; the backward reads the stored sum and one rstd a row"""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h, rstd = ops.rms_norm(x, weight, residual, eps)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.has_residual else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        if dy is None:          # only the sum is used further on
+            return dh, None, (dh if ctx.has_residual else None), None
+        dx, dw = ops.rms_norm_bwd(dy, h, weight, rstd, dh)
+        return dx, dw, (dx if ctx.has_residual else None), None
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """ops.rms_norm with autograd: -> y, or with a residual (y, h = x + residual)"""
+    return _RmsNorm.apply(x, weight, residual, eps)

@@ -13,7 +13,7 @@ per-link bound (a ring moves 2(W-1)/W x 52 MB per GPU), instead of one small col
 """
 import torch
 
-from . import losses, metric
+from . import losses, metric, ops
 
 
 def flatten_grads(params):
@@ -61,7 +61,8 @@ def broadcast_buffers(model, dist, world, src=0):
 
 
 class Trainer:
-    def __init__(self, model, lr=1e-4, weight_decay=1e-4, welsch_alpha=10.0, welsch_top_k=512, dist=None, world=1, loss_scale=None, graph=False):
+    def __init__(self, model, lr=1e-4, weight_decay=1e-4, welsch_alpha=10.0, welsch_top_k=512, dist=None, world=1, loss_scale=None, graph=False,
+                 max_grad_norm=None):
         """lr / alpha / top_k defaults: configs/cfgs.py:55,41,44; weight decay: train.py:199.
         graph=True: forward + loss + backward of a step -- about 2500 kernel launches, whose enqueueing on the host takes as long as the GPU needs to run
         them -- are recorded ONCE per input shape into a HIP graph (after `graph_warmup` eager steps) and replayed with one launch per step; the inputs
@@ -71,7 +72,12 @@ class Trainer:
         optimizer; both exact in fp32).  It exists for the fp16x3 engine's backward GEMMs, whose operands are split into
         binary16 terms: unscaled activation gradients (1e-6 .. 0.2) would fall into binary16's subnormal range.  Default
         2^16 with precision "f16x3", 1 with "f32".  If a scaled gradient exceeds 65504 the engine raises its overflow flag:
-        the step is skipped and the scale halved."""
+        the step is skipped and the scale halved.
+        max_grad_norm: a limit for the global norm of the (all-reduced, un-scaled) gradients; a larger one is scaled down to it before the optimizer, in the same pass
+        that un-scales (ops.clip_grads_).  step() then also returns "grad_norm", the norm before clipping, a scalar on the device.  None: no norm is formed."""
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError("max_grad_norm must be None or a number that is not negative, got %r" % (max_grad_norm,))
+        self.max_grad_norm = max_grad_norm
         self.model, self.dist, self.world = model, dist, world
         self.alpha, self.top_k = welsch_alpha, welsch_top_k
         self.optimizer = torch.optim.Adam(model.parameters(), lr=lr, weight_decay=weight_decay)
@@ -195,6 +201,7 @@ class Trainer:
             out, loss, parts, fwd_flag, flag = self._traced(src, tgt, transform_gt, src_overlap, tgt_overlap, fps_starts, self.loss_scale)
         fwd_hit, bwd_hit = self._overflow_hits(fwd_flag, flag)
         overflowed = fwd_hit or bwd_hit
+        grad_norm = None
         if fwd_hit:
             # |activation| > 65504 in the FORWARD: its outputs and every gradient derived from them are built on clamped values.  The loss scale cannot
             # cure that (it only lifts small gradients): skip the step without touching the scale, and give up when it persists.
@@ -218,7 +225,11 @@ class Trainer:
                 self.loss_scale = min(self.initial_loss_scale, self.loss_scale * 2.0)
                 self._clean_steps = 0
             allreduce_gradients(self.model, self.dist, self.world)
-            if self._backward_scale != 1.0:
+            if self.max_grad_norm is not None:
+                grads = [p.grad for p in self.model.parameters() if p.grad is not None]
+                if grads:
+                    grad_norm = ops.clip_grads_(grads, self.max_grad_norm, inv_scale=1.0 / self._backward_scale)
+            elif self._backward_scale != 1.0:
                 grads = [p.grad for p in self.model.parameters() if p.grad is not None]
                 torch._foreach_mul_(grads, 1.0 / self._backward_scale)          # one multi-tensor launch instead of 150 small ones
             self.optimizer.step()
@@ -227,7 +238,10 @@ class Trainer:
             B = src.shape[0]
             r_err = metric.rotation_error(out[0], transform_gt[:, :3, :3]).mean()
             t_err = metric.translation_error(out[1], transform_gt[:, :3, 3].reshape(B, 3)).mean()
-        return {"loss": loss, "skipped": overflowed, "parts": parts, "r_err_deg": r_err, "t_err": t_err, "out": out}
+        info = {"loss": loss, "skipped": overflowed, "parts": parts, "r_err_deg": r_err, "t_err": t_err, "out": out}
+        if grad_norm is not None:
+            info["grad_norm"] = grad_norm
+        return info
 
 
 class BaselineTrainer(Trainer):
