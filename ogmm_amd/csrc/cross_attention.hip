@@ -361,93 +361,320 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a, int tile_
     if (a.lse && lane == 0) a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
 }
 
-__device__ __forceinline__ bool admitted(const Args& a, int b, int n, int len) { return n < len && (!a.key_mask || a.key_mask[b * a.mask_b + n]); }
+// ---- backward.  Two kernels form the scores again from lse: one owns query rows and sums dQ over the keys (S^T, dP^T, dQ^T: three products), one owns keys and sums dK, dV over
+// the query rows of its G heads (S, dP, dV^T, dK^T: four products); no sum crosses workgroups but where few tiles are cut into parts, which are added in their order.
+struct BwdArgs : Args {
+    int row_tiles, row_splits, key_tiles, key_splits;          // dq: tiles of 128 rows, parts of the keys; dk, dv: tiles of 128 keys, parts of the rows
+    int delta_blocks;                                          // blocks of 64 rows to a key head
+    float *lse2, *delta;                                       // [B Hkv][rows]: lse log2(e) (+inf: the row has no weights), sum of dO O
+    float* top;                                                // [B Hkv][delta_blocks]: the largest |dO| (16-bit floats with five exponent bits)
+    float *part_q, *part_k, *part_v;                           // parts in the outputs' own order
+};
 
-template <class T>
-__device__ __forceinline__ float dot(const float* __restrict__ u, const T* __restrict__ x, int d) {
-    float s = 0.0f;
-    for (int c = 0; c < d; ++c) s = fmaf(u[c], static_cast<float>(x[c]), s);
-    return s;
+__device__ __forceinline__ int64_t row_offset(const Args& a, int r, int b, int hk, int64_t sb, int64_t sn, int64_t sh) {
+    const int n = a.G == 1 ? r : r / a.G, g = r - n * a.G;
+    return b * sb + n * sn + (hk * a.G + g) * sh;
 }
 
+// four threads to a row
 template <class T>
-__global__ __launch_bounds__(256) void xattn_dq_kernel(const Args a) {
-    __shared__ float qs[4][128], gs[4][128];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = a.d;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-    if (row >= static_cast<int64_t>(a.B) * a.H * a.Nq) return;
-    const int n = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H, hk = h / (a.H / a.Hkv);
-    const T *q = static_cast<const T*>(a.q) + b * a.q_b + n * a.q_n + h * a.q_h, *g = static_cast<const T*>(a.dout) + b * a.do_b + n * a.do_n + h * a.do_h;
+__global__ __launch_bounds__(256) void xattn_delta_kernel(const BwdArgs a) {
+    __shared__ float tops[4];
+    constexpr int VEC = 16 / sizeof(T);
+    typedef T tv __attribute__((ext_vector_type(VEC)));
+    const int block = blockIdx.x % a.delta_blocks, bh = blockIdx.x / a.delta_blocks, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int r = block * 64 + (threadIdx.x >> 2);
+    float delta = 0.0f, top = 0.0f;
+    if (r < a.rows) {
+        const int n = r / a.G, g = r - n * a.G;
+        const float lse = a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n];
+        const bool there = n < clamp_len(a.q_lens, b, a.Nq) && lse != -INFINITY;
+        if (there) {
+            const T *o = static_cast<const T*>(a.o) + ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+            const T* go = static_cast<const T*>(a.dout) + b * a.do_b + n * a.do_n + (hk * a.G + g) * a.do_h;
+            for (int c = (threadIdx.x & 3) * VEC; c < a.d; c += 4 * VEC) {
+                const tv x = *reinterpret_cast<const tv*>(o + c), y = *reinterpret_cast<const tv*>(go + c);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    delta = fmaf(static_cast<float>(x[k]), static_cast<float>(y[k]), delta);
+                    top = fmaxf(top, fabsf(static_cast<float>(y[k])));
+                }
+            }
+        }
+        delta += __shfl_xor(delta, 1, 64);
+        delta += __shfl_xor(delta, 2, 64);
+        if ((threadIdx.x & 3) == 0) {
+            a.lse2[static_cast<int64_t>(bh) * a.rows + r] = there ? lse * LOG2E : INFINITY;
+            a.delta[static_cast<int64_t>(bh) * a.rows + r] = delta;
+        }
+    }
+    if constexpr (std::is_same_v<T, _Float16>) {
+        top = wave_max(top);
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+        if (threadIdx.x == 0) a.top[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    }
+}
+
+// dS as an fp16 operand: times a power of two that brings the largest |dO| of the rows that share a key head to [1, 2), so that a gradient of any size keeps its precision
+// where fp16's exponents end (fp32 and bf16 have the range)
+template <class T>
+__device__ __forceinline__ float gradient_scale(const BwdArgs& a, int bh) {
+    if constexpr (std::is_same_v<T, _Float16>) {
+        float top = 0.0f;
+        for (int i = threadIdx.x & 63; i < a.delta_blocks; i += 64) top = fmaxf(top, a.top[static_cast<int64_t>(bh) * a.delta_blocks + i]);
+        top = wave_max(top);
+        if (top > 0.0f && top < INFINITY) return __uint_as_float(static_cast<uint32_t>(254 - min(253, static_cast<int>(__float_as_uint(top) >> 23))) << 23);
+    }
+    return 1.0f;
+}
+
+// a lane's column of a result to a row of channels in memory: 16-bit four channels at once, fp32 DB
+template <class T, class M>
+__device__ __forceinline__ void store_column(T* __restrict__ out, const f32x16 (&c)[M::DB], float f, int d) {
+    if constexpr (sizeof(T) == 2) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int db = 0; db < M::DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                if (M::channel(db, i) >= d) continue;
+                t4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(c[db][i + e] * f);
+                *reinterpret_cast<t4*>(out + M::channel(db, i)) = v;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (M::channel(0, i) >= d) continue;
+#pragma unroll
+            for (int db = 0; db < M::DB; ++db) out[M::channel(db, i)] = c[db][i] * f;
+        }
+    }
+}
+template <class M>
+__device__ __forceinline__ void store_part(float* __restrict__ out, const f32x16 (&c)[M::DB], float f, int d) {
+#pragma unroll
+    for (int db = 0; db < M::DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (M::channel(db, i) < d) out[M::channel(db, i)] = c[db][i] * f;
+}
+
+template <class T, int DP>
+struct Bwd {
+    static constexpr int KT = sizeof(T) == 4 && DP > 64 ? 32 : 64;          // keys (dq) or rows (dk, dv) of a tile
+    using M = Tile<T, DP, sizeof(T) == 4 ? 16 : 32>;
+    static constexpr int CPR = M::ROW / 16, PASSES = KT * CPR / 256;
+    static constexpr int LDS = 2 * KT * M::PITCH + 2 * KT * 4;
+};
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_kernel(const BwdArgs a) {
+    using S = Bwd<T, DP>;
+    using M = typename S::M;
+    constexpr int KT = S::KT, BLOCKS = KT / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *lds_k = lds, *lds_v = lds + KT * M::PITCH;
+    const uint32_t item = item_of(a);
+    if (item >= a.items) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int split = item % a.row_splits, tile = item / a.row_splits % a.row_tiles, bh = item / a.row_splits / a.row_tiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
     const T *k = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, *v = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h;
-    const int64_t at = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + h) * d;
-    const T* o = static_cast<const T*>(a.o) + at;
-    T* dq = static_cast<T*>(a.dq) + at;
-    const float lse = a.lse[row];
-    const int len = n < clamp_len(a.q_lens, b, a.Nq) && lse != -INFINITY ? clamp_len(a.kv_lens, b, a.Nk) : 0;
-    float delta = 0.0f, s0 = 0.0f, s1 = 0.0f;
-    for (int c = lane; c < d; c += 64) {
-        qs[wave][c] = static_cast<float>(q[c]) * a.scale;
-        gs[wave][c] = static_cast<float>(g[c]);
-        if (len) delta = fmaf(gs[wave][c], static_cast<float>(o[c]), delta);
-    }
-    delta = wave_sum(delta);
-    for (int j0 = 0; j0 < len; j0 += 64) {
-        const int j = j0 + lane;
-        float ds = 0.0f;
-        if (admitted(a, b, j, len)) ds = expf(dot(qs[wave], k + j * a.k_n, d) - lse) * (dot(gs[wave], v + j * a.v_n, d) - delta);
-        for (int i = 0; i < 64 && j0 + i < len; ++i) {
-            const float si = __shfl(ds, i, 64);
-            if (si == 0.0f) continue;
-            const T* ki = k + static_cast<int64_t>(j0 + i) * a.k_n;
-            if (lane < d) s0 = fmaf(si, static_cast<float>(ki[lane]), s0);
-            if (lane + 64 < d) s1 = fmaf(si, static_cast<float>(ki[lane + 64]), s1);
+    const int row = tile * 128 + wave * 32 + (lane & 31);
+    const bool row_there = row < q_rows;
+    const float c = a.scale * LOG2E, up = gradient_scale<T>(a, bh);
+    u32x4 q[M::CHUNKS], go[M::CHUNKS];
+    float lse2 = INFINITY, delta = 0.0f;
+    {
+        const int64_t at = static_cast<int64_t>(bh) * a.rows + row;
+        if (row_there) { lse2 = a.lse2[at]; delta = a.delta[at]; }
+        const char* pq = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + row_offset(a, row, b, hk, a.q_b, a.q_n, a.q_h));
+        const char* pg = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + row_offset(a, row, b, hk, a.do_b, a.do_n, a.do_h));
+#pragma unroll
+        for (int s = 0; s < M::CHUNKS; ++s) {
+            const int at = 32 * s + 16 * (lane >> 5);
+            q[s] = go[s] = u32x4{0, 0, 0, 0};
+            if (row_there && at < a.d * static_cast<int>(sizeof(T))) {
+                q[s] = *reinterpret_cast<const u32x4*>(pq + at);
+                go[s] = *reinterpret_cast<const u32x4*>(pg + at);
+            }
         }
     }
-    if (lane < d) dq[lane] = static_cast<T>(s0 * a.scale);
-    if (lane + 64 < d) dq[lane + 64] = static_cast<T>(s1 * a.scale);
+    const int tiles = tile * 128 < q_rows ? (len + KT - 1) / KT : 0, per = (tiles + a.row_splits - 1) / a.row_splits, end = min(tiles, (split + 1) * per);
+    f32x16 dq[M::DB] = {};
+    u32x4 rk[S::PASSES], rv[S::PASSES];
+    uint64_t bits[1], next_bits = 0;
+    auto next = [&](int t) {
+        for (; t < end; ++t)
+            if ((next_bits = key_bits(a, b, t * KT, min(len, (t + 1) * KT)))) break;
+        return t;
+    };
+    int t = next(split * per);
+    if (t < end) {
+        fetch<T, S::CPR>(rk, k, a.k_n, t * KT, a.Nk, a.d);
+        fetch<T, S::CPR>(rv, v, a.v_n, t * KT, a.Nk, a.d);
+    }
+    while (t < end) {
+        bits[0] = next_bits;
+        const bool full = bits[0] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
+        put<M::PITCH, S::CPR>(lds_k, rk, bits, full);
+        put<M::PITCH, S::CPR>(lds_v, rv, bits, full);
+        __syncthreads();
+        t = next(t + 1);
+        if (t < end) {
+            fetch<T, S::CPR>(rk, k, a.k_n, t * KT, a.Nk, a.d);
+            fetch<T, S::CPR>(rv, v, a.v_n, t * KT, a.Nk, a.d);
+        }
+#pragma unroll
+        for (int j = 0; j < BLOCKS; ++j) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int u = 0; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_k, 32 * j, u), q[u], T());
+#pragma unroll
+            for (int u = 0; u < M::CHUNKS; ++u) mma(dp, M::row_chunk(lds_v, 32 * j, u), go[u], T());
+            const uint32_t mine = static_cast<uint32_t>(bits[0] >> (32 * j)) >> (4 * (lane >> 5));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2));
+                s[i] = p * (dp[i] - delta) * up;
+                if (!full && !(mine >> (8 * (i / 4) + i % 4) & 1)) s[i] = 0.0f;
+            }
+            u32x4 ds[sizeof(T) == 4 ? 4 : 2];
+            as_operand<T>(ds, s);
+            M::mul_t(dq, lds_k, 32 * j, ds);
+        }
+        __syncthreads();
+    }
+    if (row >= a.rows) return;
+    const int n = row / a.G, g = row - n * a.G;
+    const int64_t at = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+    const float f = a.scale / up;
+    if (a.row_splits > 1) store_part<M>(a.part_q + split * (static_cast<int64_t>(a.B) * a.Nq * a.H * a.d) + at, dq, f, a.d);
+    else store_column<T, M>(static_cast<T*>(a.dq) + at, dq, f, a.d);
 }
 
-// rows of k and v: waves over (b, hk, j); a key's sum runs over the query heads that share it
+// rows [r0, r0 + KT) of q or dout
+template <class T, int CPR, int PASSES>
+__device__ __forceinline__ void fetch_rows(u32x4 (&x)[PASSES], const Args& a, const void* p, int64_t sb, int64_t sn, int64_t sh, int r0, int b, int hk) {
+    const int c = threadIdx.x % CPR;
+    const bool there = c * 16 < a.d * static_cast<int>(sizeof(T));
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int r = min(r0 + static_cast<int>(threadIdx.x) / CPR + i * (256 / CPR), a.rows - 1);
+        x[i] = u32x4{0, 0, 0, 0};
+        if (there) x[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(static_cast<const T*>(p) + row_offset(a, r, b, hk, sb, sn, sh)) + 16 * c);
+    }
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv_kernel(const BwdArgs a) {
+    using S = Bwd<T, DP>;
+    using M = typename S::M;
+    constexpr int QT = S::KT, BLOCKS = QT / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char *lds_q = lds, *lds_g = lds + QT * M::PITCH;
+    float *lds_lse = reinterpret_cast<float*>(lds + 2 * QT * M::PITCH), *lds_delta = lds_lse + QT;
+    const uint32_t item = item_of(a);
+    if (item >= a.items) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int split = item % a.key_splits, tile = item / a.key_splits % a.key_tiles, bh = item / a.key_splits / a.key_tiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
+    const int key = tile * 128 + wave * 32 + (lane & 31);
+    const bool key_there = key < len && (!a.key_mask || a.key_mask[b * a.mask_b + key]);
+    // (all four waves take part in the tiles of rows, or none: a tile of keys without one that is admitted)
+    const bool any = (key_bits(a, b, tile * 128, len) | key_bits(a, b, tile * 128 + 64, len)) != 0;
+    const float c = a.scale * LOG2E, up = gradient_scale<T>(a, bh);
+    u32x4 k[M::CHUNKS], v[M::CHUNKS];
+    {
+        const char* pk = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + b * a.k_b + key * a.k_n + hk * a.k_h);
+        const char* pv = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + b * a.v_b + key * a.v_n + hk * a.v_h);
+#pragma unroll
+        for (int s = 0; s < M::CHUNKS; ++s) {
+            const int at = 32 * s + 16 * (lane >> 5);
+            k[s] = v[s] = u32x4{0, 0, 0, 0};
+            if (key_there && at < a.d * static_cast<int>(sizeof(T))) {
+                k[s] = *reinterpret_cast<const u32x4*>(pk + at);
+                v[s] = *reinterpret_cast<const u32x4*>(pv + at);
+            }
+        }
+    }
+    const int tiles = any ? (q_rows + QT - 1) / QT : 0, per = (tiles + a.key_splits - 1) / a.key_splits, end = min(tiles, (split + 1) * per);
+    f32x16 dk[M::DB] = {}, dv[M::DB] = {};
+    u32x4 rq[S::PASSES], rg[S::PASSES];
+    float r_stat = 0.0f;          // threads 0 .. QT: a row's lse, QT .. 2 QT: its delta
+    auto fetch_tile = [&](int t) {
+        fetch_rows<T, S::CPR>(rq, a, a.q, a.q_b, a.q_n, a.q_h, t * QT, b, hk);
+        fetch_rows<T, S::CPR>(rg, a, a.dout, a.do_b, a.do_n, a.do_h, t * QT, b, hk);
+        const int r = t * QT + threadIdx.x % QT;
+        if (threadIdx.x < 2 * QT) r_stat = r < q_rows ? (threadIdx.x < QT ? a.lse2 : a.delta)[static_cast<int64_t>(bh) * a.rows + r] : threadIdx.x < QT ? INFINITY : 0.0f;
+    };
+    int t = split * per;
+    if (t < end) fetch_tile(t);
+    for (; t < end; ++t) {
+        const int left = q_rows - t * QT;
+        const uint64_t bits[1] = {left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1};          // rows behind q_lens become zeros
+        const bool full = left >= QT;
+        put<M::PITCH, S::CPR>(lds_q, rq, bits, full);
+        put<M::PITCH, S::CPR>(lds_g, rg, bits, full);
+        if (threadIdx.x < 2 * QT) lds_lse[threadIdx.x] = r_stat;
+        __syncthreads();
+        if (t + 1 < end) fetch_tile(t + 1);
+#pragma unroll
+        for (int j = 0; j < BLOCKS; ++j) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int u = 0; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_q, 32 * j, u), k[u], T());
+#pragma unroll
+            for (int u = 0; u < M::CHUNKS; ++u) mma(dp, M::row_chunk(lds_g, 32 * j, u), v[u], T());
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int r = 32 * j + 2 * i + 4 * (lane >> 5);          // result row 8 (i / 4) + 4 (lane / 32) + i % 4
+                const float4 l4 = *reinterpret_cast<const float4*>(lds_lse + r), d4 = *reinterpret_cast<const float4*>(lds_delta + r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[i + e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], c, -(&l4.x)[e]));
+                    dp[i + e] = s[i + e] * (dp[i + e] - (&d4.x)[e]) * up;
+                }
+            }
+            u32x4 y[sizeof(T) == 4 ? 4 : 2];
+            as_operand<T>(y, s);
+            M::mul_t(dv, lds_g, 32 * j, y);
+            as_operand<T>(y, dp);
+            M::mul_t(dk, lds_q, 32 * j, y);
+        }
+        __syncthreads();
+    }
+    if (key >= a.Nk) return;
+    // (a key that is not admitted has gathered the weights that its zeros gave it: nobody else's sum; its gradient is zero)
+    const int64_t at = ((static_cast<int64_t>(b) * a.Nk + key) * a.Hkv + hk) * a.d, all = static_cast<int64_t>(a.B) * a.Nk * a.Hkv * a.d;
+    if (!key_there)
+#pragma unroll
+        for (int db = 0; db < M::DB; ++db) dk[db] = dv[db] = f32x16{};
+    if (a.key_splits > 1) {
+        store_part<M>(a.part_k + split * all + at, dk, a.scale / up, a.d);
+        store_part<M>(a.part_v + split * all + at, dv, 1.0f, a.d);
+    } else {
+        store_column<T, M>(static_cast<T*>(a.dk) + at, dk, a.scale / up, a.d);
+        store_column<T, M>(static_cast<T*>(a.dv) + at, dv, 1.0f, a.d);
+    }
+}
+
+// out = the parts' sum, in their order (n: a multiple of 8 values)
 template <class T>
-__global__ __launch_bounds__(256) void xattn_dkv_kernel(const Args a) {
-    __shared__ float ks[4][128], vs[4][128];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = a.d;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-    if (row >= static_cast<int64_t>(a.B) * a.Hkv * a.Nk) return;
-    const int j = row % a.Nk, hk = row / a.Nk % a.Hkv, b = row / a.Nk / a.Hkv, G = a.H / a.Hkv;
-    const T *k = static_cast<const T*>(a.k) + b * a.k_b + j * a.k_n + hk * a.k_h, *v = static_cast<const T*>(a.v) + b * a.v_b + j * a.v_n + hk * a.v_h;
-    const int rows = admitted(a, b, j, clamp_len(a.kv_lens, b, a.Nk)) ? clamp_len(a.q_lens, b, a.Nq) : 0;
-    for (int c = lane; c < d; c += 64) {
-        ks[wave][c] = static_cast<float>(k[c]) * a.scale;
-        vs[wave][c] = static_cast<float>(v[c]);
+__global__ __launch_bounds__(256) void xattn_add_kernel(const float* __restrict__ part, int parts, int64_t n, T* __restrict__ out) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    float4 x = *reinterpret_cast<const float4*>(part + i);
+    for (int s = 1; s < parts; ++s) {
+        const float4 y = *reinterpret_cast<const float4*>(part + s * n + i);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-    float k0 = 0.0f, k1 = 0.0f, v0 = 0.0f, v1 = 0.0f;
-    for (int h = hk * G; h < (hk + 1) * G; ++h)
-        for (int n0 = 0; n0 < rows; n0 += 64) {
-            const int n = n0 + lane;
-            float p = 0.0f, ds = 0.0f;
-            if (n < rows) {
-                const T *q = static_cast<const T*>(a.q) + b * a.q_b + n * a.q_n + h * a.q_h, *g = static_cast<const T*>(a.dout) + b * a.do_b + n * a.do_n + h * a.do_h;
-                const T* o = static_cast<const T*>(a.o) + ((static_cast<int64_t>(b) * a.Nq + n) * a.H + h) * d;
-                float delta = 0.0f;
-                for (int c = 0; c < d; ++c) delta = fmaf(static_cast<float>(g[c]), static_cast<float>(o[c]), delta);
-                p = expf(dot(ks[wave], q, d) - a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Nq + n]);
-                ds = p * (dot(vs[wave], g, d) - delta);
-            }
-            for (int i = 0; i < 64 && n0 + i < rows; ++i) {
-                const float pi = __shfl(p, i, 64), si = __shfl(ds, i, 64);
-                const T *q = static_cast<const T*>(a.q) + b * a.q_b + (n0 + i) * a.q_n + h * a.q_h;
-                const T *g = static_cast<const T*>(a.dout) + b * a.do_b + (n0 + i) * a.do_n + h * a.do_h;
-                if (lane < d) { v0 = fmaf(pi, static_cast<float>(g[lane]), v0); k0 = fmaf(si, static_cast<float>(q[lane]), k0); }
-                if (lane + 64 < d) { v1 = fmaf(pi, static_cast<float>(g[lane + 64]), v1); k1 = fmaf(si, static_cast<float>(q[lane + 64]), k1); }
-            }
-        }
-    const int64_t at = ((static_cast<int64_t>(b) * a.Nk + j) * a.Hkv + hk) * d;
-    T *dk = static_cast<T*>(a.dk) + at, *dv = static_cast<T*>(a.dv) + at;
-    if (lane < d) { dk[lane] = static_cast<T>(k0 * a.scale); dv[lane] = static_cast<T>(v0); }
-    if (lane + 64 < d) { dk[lane + 64] = static_cast<T>(k1 * a.scale); dv[lane + 64] = static_cast<T>(v1); }
+    *reinterpret_cast<t4*>(out + i) = t4{static_cast<T>(x.x), static_cast<T>(x.y), static_cast<T>(x.z), static_cast<T>(x.w)};
 }
-
 
 // ---- host
 template <class F>
@@ -501,6 +728,64 @@ int launch_fwd(const Args& a, hipStream_t stream) {
     return check_launch("ogmm_xattn_fwd");
 }
 
+BwdArgs backward_args(const ogmm_xattn* x, float* ws, int64_t* floats) {
+    BwdArgs a{};
+    static_cast<ogmm_xattn&>(a) = *x;
+    a.G = a.H / a.Hkv;
+    a.rows = a.Nq * a.G;
+    const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
+    a.row_tiles = (a.rows + 127) / 128;
+    a.key_tiles = (a.Nk + 127) / 128;
+    a.delta_blocks = (a.rows + 63) / 64;
+    // as in the forward: parts where the tiles alone leave CUs without work, of 256 keys or rows at least
+    auto parts = [&](int64_t tiles, int64_t n) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), (n + 255) / 256))); };
+    a.row_splits = parts(heads * a.row_tiles, a.Nk);
+    a.key_splits = parts(heads * a.key_tiles, a.rows);
+    int64_t n = 0;
+    auto take = [&](int64_t count) {
+        float* at = ws ? ws + n : nullptr;
+        n += (count + 3) / 4 * 4;
+        return at;
+    };
+    a.lse2 = take(heads * a.rows);
+    a.delta = take(heads * a.rows);
+    a.top = take(heads * a.delta_blocks);
+    if (a.row_splits > 1) a.part_q = take(a.row_splits * (heads * a.rows * a.d));
+    if (a.key_splits > 1) {
+        a.part_k = take(a.key_splits * (heads * a.Nk * a.d));
+        a.part_v = take(a.key_splits * (heads * a.Nk * a.d));
+    }
+    *floats = n;
+    return a;
+}
+
+template <class T, int DP>
+int launch_bwd(BwdArgs a, hipStream_t stream) {
+    using S = Bwd<T, DP>;
+    static_assert(S::LDS <= 65536, "LDS");
+    const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
+    auto add = [&](const float* part, int parts, int64_t n, void* out) {
+        xattn_add_kernel<T><<<static_cast<uint32_t>((n / 4 + 255) / 256), 256, 0, stream>>>(part, parts, n, static_cast<T*>(out));
+    };
+    if (a.Nq) {
+        xattn_delta_kernel<T><<<static_cast<uint32_t>(heads * a.delta_blocks), 256, 0, stream>>>(a);
+        a.items = static_cast<uint32_t>(heads * a.row_tiles * a.row_splits);
+        a.per_xcd = (a.items + 7) / 8;
+        xattn_dq_kernel<T, DP><<<a.per_xcd * 8, 256, S::LDS, stream>>>(a);
+        if (a.row_splits > 1) add(a.part_q, a.row_splits, heads * a.rows * a.d, a.dq);
+    }
+    if (a.Nk) {
+        a.items = static_cast<uint32_t>(heads * a.key_tiles * a.key_splits);
+        a.per_xcd = (a.items + 7) / 8;
+        xattn_dkv_kernel<T, DP><<<a.per_xcd * 8, 256, S::LDS, stream>>>(a);
+        if (a.key_splits > 1) {
+            add(a.part_k, a.key_splits, heads * a.Nk * a.d, a.dk);
+            add(a.part_v, a.key_splits, heads * a.Nk * a.d, a.dv);
+        }
+    }
+    return check_launch("ogmm_xattn_bwd");
+}
+
 int check(const char* who, const ogmm_xattn* a) {
     OGMM_REQUIRE(a, "%s: missing argument", who);
     OGMM_REQUIRE(a->B >= 0 && a->Nq >= 0 && a->Nk >= 0 && a->H >= 1 && a->Hkv >= 1, "%s: B = %d, Nq = %d, Nk = %d, H = %d, Hkv = %d", who, a->B, a->Nq, a->Nk, a->H, a->Hkv);
@@ -523,7 +808,12 @@ int check(const char* who, const ogmm_xattn* a) {
 }  // namespace
 
 extern "C" int64_t ogmm_xattn_workspace_bytes(const ogmm_xattn* a, int backward) {
-    if (!a || a->B < 1 || a->Nq < 1 || a->Nk < 0 || a->H < 1 || a->Hkv < 1 || backward) return 0;
+    if (!a || a->B < 1 || a->Nq < 0 || a->Nk < 0 || a->H < 1 || a->Hkv < 1 || a->H < a->Hkv) return 0;
+    if (backward) {
+        int64_t floats;
+        backward_args(a, nullptr, &floats);
+        return floats * static_cast<int64_t>(sizeof(float));
+    }
     const Args f = forward_args(a, nullptr);
     return f.splits > 1 ? static_cast<int64_t>(f.items) * (few_rows(a) ? 32 : 128) * (a->d + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
@@ -552,9 +842,10 @@ extern "C" int ogmm_xattn_bwd(const ogmm_xattn* a, void* stream) {
     OGMM_REQUIRE(!rows || (a->dout && a->lse && a->dq), "ogmm_xattn_bwd: missing argument");
     OGMM_REQUIRE(!keys || (a->dk && a->dv), "ogmm_xattn_bwd: missing argument");
     if (!rows && !keys) return 0;
+    int64_t floats;
+    const BwdArgs args = backward_args(a, static_cast<float*>(a->workspace), &floats);
+    OGMM_REQUIRE(!floats || (a->workspace && aligned16(a->workspace)), "ogmm_xattn_bwd: missing workspace");
     return with_type(a->type, [&](auto t) {
-        if (rows) xattn_dq_kernel<decltype(t)><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, as_stream(stream)>>>([&] { Args g{}; static_cast<ogmm_xattn&>(g) = *a; return g; }());
-        if (keys) xattn_dkv_kernel<decltype(t)><<<static_cast<uint32_t>((keys + 3) / 4), 256, 0, as_stream(stream)>>>([&] { Args g{}; static_cast<ogmm_xattn&>(g) = *a; return g; }());
-        return check_launch("ogmm_xattn_bwd");
+        return with_width(a->d, [&](auto w) { return launch_bwd<decltype(t), decltype(w)::value>(args, as_stream(stream)); });
     });
 }
