@@ -49,7 +49,7 @@ class XattnDesc(Structure):
         ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
         ("q_b", c_int64), ("q_n", c_int64), ("q_h", c_int64), ("k_b", c_int64), ("k_n", c_int64), ("k_h", c_int64),
         ("v_b", c_int64), ("v_n", c_int64), ("v_h", c_int64),
-        ("o", c_void_p), ("lse", c_void_p),
+        ("o", c_void_p), ("rest", c_void_p), ("lse", c_void_p),
         ("B", c_int32), ("Nq", c_int32), ("Nk", c_int32), ("H", c_int32), ("Hkv", c_int32), ("d", c_int32), ("type", c_int32),
         ("scale", c_float),
         ("q_lens", c_void_p), ("kv_lens", c_void_p), ("key_mask", c_void_p), ("mask_b", c_int64),

@@ -26,15 +26,19 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 struct Args : ogmm_xattn {
     int G, rows;                   // query heads to a key head, query rows to a key head (Nq G)
     int tiles, splits;             // row tiles, parts of the keys
-    uint32_t items, per_xcd;       // workgroups in all, and of one XCD
+    uint32_t items, run;           // workgroups that have work, and neighbours among them that one XCD takes
     float* part;                   // splits > 1: [items of a split][rows of a tile][d] sums and, behind them, (maximum, sum) pairs
     float* part_ml;
 };
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int n) { return lens ? max(0, min(n, lens[b])) : n; }
 
-// Workgroups go to the XCDs in turn; those of one (batch, key head) read the same keys, so each XCD gets a run of neighbours for its own L2
-__device__ __forceinline__ uint32_t item_of(const Args& a) { return blockIdx.x % 8 * a.per_xcd + blockIdx.x / 8; }
+// Workgroups go to the XCDs in turn.  Tiles of one (batch, key head) read the same keys, so an XCD gets runs of neighbours for its own L2; runs are dealt in turn, and so
+// short (at least 64 of them where there are that many tiles) that batch entries of different lengths come out even.
+__device__ __forceinline__ uint32_t item_of(const Args& a) {
+    const uint32_t xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+    return (at / a.run * 8 + xcd) * a.run + at % a.run;
+}
 
 // ---- products of 32x32 tiles, sixteen bytes of either operand to a lane: row lane % 32, byte 16 (lane / 32) of a 32-byte chunk of the contraction
 __device__ __forceinline__ void mma(f32x16& c, u32x4 a, u32x4 b, __bf16) {
@@ -116,6 +120,50 @@ __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 
 __device__ __forceinline__ uint64_t key_bits(const Args& a, int b, int n0, int len) {
     const int n = n0 + (threadIdx.x & 63);
     return __ballot(n < len && (!a.key_mask || a.key_mask[b * a.mask_b + n]));
+}
+
+// a lane's column of a result times f to a row of channels in memory: 16-bit four channels at once, fp32 DB.  rest: what the rounding to 16 bits left, in 16 bits again
+template <class T, class M>
+__device__ __forceinline__ void store_column(T* __restrict__ out, T* __restrict__ rest, const f32x16 (&c)[M::DB], float f, int d) {
+    if constexpr (sizeof(T) == 2) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int db = 0; db < M::DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                if (M::channel(db, i) >= d) continue;
+                t4 v, w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = c[db][i + e] * f;
+                    v[e] = static_cast<T>(x);
+                    w[e] = static_cast<T>(x - static_cast<float>(v[e]));
+                }
+                *reinterpret_cast<t4*>(out + M::channel(db, i)) = v;
+                if (rest) *reinterpret_cast<t4*>(rest + M::channel(db, i)) = w;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (M::channel(0, i) >= d) continue;
+#pragma unroll
+            for (int db = 0; db < M::DB; ++db) out[M::channel(db, i)] = c[db][i] * f;
+        }
+    }
+}
+template <class M>
+__device__ __forceinline__ void store_part(float* __restrict__ out, const f32x16 (&c)[M::DB], float f, int d) {
+#pragma unroll
+    for (int db = 0; db < M::DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (M::channel(db, i) < d) out[M::channel(db, i)] = c[db][i] * f;
+}
+template <class T>
+__device__ __forceinline__ void store_one(const ogmm_xattn& a, int64_t at, float x) {
+    const T v = static_cast<T>(x);
+    static_cast<T*>(a.o)[at] = v;
+    if (sizeof(T) == 2 && a.rest) static_cast<T*>(a.rest)[at] = static_cast<T>(x - static_cast<float>(v));
 }
 
 template <class T, int DP, bool KEY_WAVES>
@@ -296,13 +344,13 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
             const int on = out_row / a.G, og = out_row - on * a.G;
             const float inv = a.splits > 1 ? 1.0f : all.y > 0.0f ? 1.0f / all.y : all.y;
             float* part = a.splits > 1 ? a.part + (static_cast<int64_t>(item) * 32 + r) * a.d : nullptr;
-            T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(b) * a.Nq + on) * a.H + hk * a.G + og) * a.d;
+            const int64_t out = ((static_cast<int64_t>(b) * a.Nq + on) * a.H + hk * a.G + og) * a.d;
             for (int ch = threadIdx.x & 7; ch < a.d; ch += 8) {
                 float x = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) x += sums[(w * 32 + r) * (DP + 4) + ch];
                 if (part) part[ch] = x;
-                else out[ch] = static_cast<T>(x * inv);
+                else store_one<T>(a, out + ch, x * inv);
             }
             if ((threadIdx.x & 7) == 0) {
                 if (a.splits > 1) reinterpret_cast<float2*>(a.part_ml)[static_cast<int64_t>(item) * 32 + r] = all;
@@ -312,22 +360,12 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
     } else {
         if (row >= a.rows) return;
         if (a.splits > 1) {
-            float* part = a.part + (static_cast<int64_t>(item) * S::ROWS + wave * 32 + (lane & 31)) * a.d;
             if (lane < 32) reinterpret_cast<float2*>(a.part_ml)[static_cast<int64_t>(item) * S::ROWS + wave * 32 + lane] = make_float2(m, l);
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (K::channel(db, i) < a.d) part[K::channel(db, i)] = o[db][i];
+            store_part<K>(a.part + (static_cast<int64_t>(item) * S::ROWS + wave * 32 + (lane & 31)) * a.d, o, 1.0f, a.d);
             return;
         }
-        const float inv = l > 0.0f ? 1.0f / l : l;
-        T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (K::channel(db, i) < a.d) out[K::channel(db, i)] = static_cast<T>(o[db][i] * inv);
+        const int64_t out = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+        store_column<T, K>(static_cast<T*>(a.o) + out, a.rest ? static_cast<T*>(a.rest) + out : nullptr, o, l > 0.0f ? 1.0f / l : l, a.d);
         if (a.lse && lane < 32) a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
     }
 }
@@ -355,9 +393,9 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a, int tile_
         if (lane + 64 < a.d) o1 = fmaf(a.part[at * a.d + lane + 64], f, o1);
     }
     const float inv = l > 0.0f ? 1.0f / l : l;
-    T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
-    if (lane < a.d) out[lane] = static_cast<T>(o0 * inv);
-    if (lane + 64 < a.d) out[lane + 64] = static_cast<T>(o1 * inv);
+    const int64_t out = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+    if (lane < a.d) store_one<T>(a, out + lane, o0 * inv);
+    if (lane + 64 < a.d) store_one<T>(a, out + lane + 64, o1 * inv);
     if (a.lse && lane == 0) a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n] = l == 0.0f ? -INFINITY : (top + log2f(l)) * LN2;
 }
 
@@ -390,13 +428,16 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(const BwdArgs a) {
         const float lse = a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n];
         const bool there = n < clamp_len(a.q_lens, b, a.Nq) && lse != -INFINITY;
         if (there) {
-            const T *o = static_cast<const T*>(a.o) + ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+            const int64_t at = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+            const T *o = static_cast<const T*>(a.o) + at, *rest = sizeof(T) == 2 && a.rest ? static_cast<const T*>(a.rest) + at : nullptr;
             const T* go = static_cast<const T*>(a.dout) + b * a.do_b + n * a.do_n + (hk * a.G + g) * a.do_h;
             for (int c = (threadIdx.x & 3) * VEC; c < a.d; c += 4 * VEC) {
                 const tv x = *reinterpret_cast<const tv*>(o + c), y = *reinterpret_cast<const tv*>(go + c);
+                tv z = {};
+                if (rest) z = *reinterpret_cast<const tv*>(rest + c);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    delta = fmaf(static_cast<float>(x[k]), static_cast<float>(y[k]), delta);
+                    delta = fmaf(static_cast<float>(x[k]) + static_cast<float>(z[k]), static_cast<float>(y[k]), delta);
                     top = fmaxf(top, fabsf(static_cast<float>(y[k])));
                 }
             }
@@ -427,39 +468,6 @@ __device__ __forceinline__ float gradient_scale(const BwdArgs& a, int bh) {
         if (top > 0.0f && top < INFINITY) return __uint_as_float(static_cast<uint32_t>(254 - min(253, static_cast<int>(__float_as_uint(top) >> 23))) << 23);
     }
     return 1.0f;
-}
-
-// a lane's column of a result to a row of channels in memory: 16-bit four channels at once, fp32 DB
-template <class T, class M>
-__device__ __forceinline__ void store_column(T* __restrict__ out, const f32x16 (&c)[M::DB], float f, int d) {
-    if constexpr (sizeof(T) == 2) {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-        for (int db = 0; db < M::DB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                if (M::channel(db, i) >= d) continue;
-                t4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(c[db][i + e] * f);
-                *reinterpret_cast<t4*>(out + M::channel(db, i)) = v;
-            }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (M::channel(0, i) >= d) continue;
-#pragma unroll
-            for (int db = 0; db < M::DB; ++db) out[M::channel(db, i)] = c[db][i] * f;
-        }
-    }
-}
-template <class M>
-__device__ __forceinline__ void store_part(float* __restrict__ out, const f32x16 (&c)[M::DB], float f, int d) {
-#pragma unroll
-    for (int db = 0; db < M::DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (M::channel(db, i) < d) out[M::channel(db, i)] = c[db][i] * f;
 }
 
 template <class T, int DP>
@@ -553,7 +561,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
     const int64_t at = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
     const float f = a.scale / up;
     if (a.row_splits > 1) store_part<M>(a.part_q + split * (static_cast<int64_t>(a.B) * a.Nq * a.H * a.d) + at, dq, f, a.d);
-    else store_column<T, M>(static_cast<T*>(a.dq) + at, dq, f, a.d);
+    else store_column<T, M>(static_cast<T*>(a.dq) + at, nullptr, dq, f, a.d);
 }
 
 // rows [r0, r0 + KT) of q or dout
@@ -657,8 +665,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
         store_part<M>(a.part_k + split * all + at, dk, a.scale / up, a.d);
         store_part<M>(a.part_v + split * all + at, dv, 1.0f, a.d);
     } else {
-        store_column<T, M>(static_cast<T*>(a.dk) + at, dk, a.scale / up, a.d);
-        store_column<T, M>(static_cast<T*>(a.dv) + at, dv, 1.0f, a.d);
+        store_column<T, M>(static_cast<T*>(a.dk) + at, nullptr, dk, a.scale / up, a.d);
+        store_column<T, M>(static_cast<T*>(a.dv) + at, nullptr, dv, 1.0f, a.d);
     }
 }
 
@@ -695,6 +703,14 @@ int with_width(int d, F&& f) {
 // Up to 32 query rows of a key head (single tokens): one row tile, and the four waves of its workgroup take different keys.
 bool few_rows(const ogmm_xattn* a) { return static_cast<int64_t>(a->Nq) * (a->H / a->Hkv) <= 32; }
 
+// -> the grid; per_head: the workgroups of one key head
+uint32_t deal(Args& a, int64_t items, int64_t per_head) {
+    a.items = static_cast<uint32_t>(items);
+    a.run = static_cast<uint32_t>(std::max<int64_t>(1, std::min(per_head, items / 64)));
+    const uint32_t runs = (a.items + a.run - 1) / a.run;
+    return (runs + 7) / 8 * 8 * a.run;
+}
+
 Args forward_args(const ogmm_xattn* x, float* ws) {
     Args a{};
     static_cast<ogmm_xattn&>(a) = *x;
@@ -706,21 +722,21 @@ Args forward_args(const ogmm_xattn* x, float* ws) {
     const int64_t base = static_cast<int64_t>(a.B) * a.Hkv * a.tiles;
     a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(base, 1), (a.Nk + 255) / 256)));
     a.items = static_cast<uint32_t>(base * a.splits);
-    a.per_xcd = (a.items + 7) / 8;
     a.part_ml = ws;
     a.part = ws ? ws + static_cast<int64_t>(a.items) * tile_rows * 2 : nullptr;
     return a;
 }
 
 template <class T, int DP, bool KEY_WAVES>
-int launch_fwd(const Args& a, hipStream_t stream) {
+int launch_fwd(Args a, hipStream_t stream) {
     using S = Fwd<T, DP, KEY_WAVES>;
     if constexpr (S::LDS > 65536) {
         static PerDeviceOnce once;
         if (once.first() && hipFuncSetAttribute(reinterpret_cast<const void*>(&xattn_fwd_kernel<T, DP, KEY_WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess)
             return fail("ogmm_xattn_fwd: %d bytes of LDS are not available", S::LDS);
     }
-    xattn_fwd_kernel<T, DP, KEY_WAVES><<<a.per_xcd * 8, 256, S::LDS, stream>>>(a);
+    const uint32_t grid = deal(a, a.items, static_cast<int64_t>(a.tiles) * a.splits);
+    xattn_fwd_kernel<T, DP, KEY_WAVES><<<grid, 256, S::LDS, stream>>>(a);
     if (a.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.rows;
         xattn_join_kernel<T><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, stream>>>(a, S::ROWS);
@@ -769,15 +785,13 @@ int launch_bwd(BwdArgs a, hipStream_t stream) {
     };
     if (a.Nq) {
         xattn_delta_kernel<T><<<static_cast<uint32_t>(heads * a.delta_blocks), 256, 0, stream>>>(a);
-        a.items = static_cast<uint32_t>(heads * a.row_tiles * a.row_splits);
-        a.per_xcd = (a.items + 7) / 8;
-        xattn_dq_kernel<T, DP><<<a.per_xcd * 8, 256, S::LDS, stream>>>(a);
+        const uint32_t grid = deal(a, heads * a.row_tiles * a.row_splits, static_cast<int64_t>(a.row_tiles) * a.row_splits);
+        xattn_dq_kernel<T, DP><<<grid, 256, S::LDS, stream>>>(a);
         if (a.row_splits > 1) add(a.part_q, a.row_splits, heads * a.rows * a.d, a.dq);
     }
     if (a.Nk) {
-        a.items = static_cast<uint32_t>(heads * a.key_tiles * a.key_splits);
-        a.per_xcd = (a.items + 7) / 8;
-        xattn_dkv_kernel<T, DP><<<a.per_xcd * 8, 256, S::LDS, stream>>>(a);
+        const uint32_t grid = deal(a, heads * a.key_tiles * a.key_splits, static_cast<int64_t>(a.key_tiles) * a.key_splits);
+        xattn_dkv_kernel<T, DP><<<grid, 256, S::LDS, stream>>>(a);
         if (a.key_splits > 1) {
             add(a.part_k, a.key_splits, heads * a.Nk * a.d, a.dk);
             add(a.part_v, a.key_splits, heads * a.Nk * a.d, a.dv);
@@ -795,7 +809,7 @@ int check(const char* who, const ogmm_xattn* a) {
     const int64_t e = a->type == OGMM_F32 ? 4 : 2;
     const int64_t strides[] = {a->q_b, a->q_n, a->q_h, a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h};
     for (int64_t s : strides) OGMM_REQUIRE(s * e % 16 == 0, "%s: a stride of %lld elements is not a multiple of 16 bytes", who, static_cast<long long>(s));
-    OGMM_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o), "%s: addresses must be multiples of 16 bytes", who);
+    OGMM_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->rest), "%s: addresses must be multiples of 16 bytes", who);
     OGMM_REQUIRE(isfinite(a->scale), "%s: scale must be finite", who);
     // (a workgroup takes several rows, so this keeps every grid below 2^31 workgroups and a row's number within 32 bits)
     OGMM_REQUIRE(static_cast<double>(a->B) * a->H * a->Nq < 2147483648.0 && static_cast<double>(a->B) * a->Hkv * a->Nk < 2147483648.0, "%s: more than 2^31 rows", who);

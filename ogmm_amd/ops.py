@@ -1258,30 +1258,35 @@ def _xattn_call(name, a, dev, backward):
     _call_on(dev, name, ctypes.byref(a))
 
 
-def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=None, need_lse=False):
+def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=None, need_lse=False, need_rest=False):
     """Attention of query rows to states of another sequence: softmax(scale q k^T) v over each row's admitted keys.
     q [B, Nq, H, d]; k, v [B, Nk, Hkv, d], H a multiple of Hkv (query head j reads key head j // (H // Hkv)); d a multiple of 8 up to 128; float32, bfloat16 or
     float16, any strides (channels contiguous and 16-byte steps are taken as they are, anything else is copied).  kv_lens / q_lens int32 [B]: how many of the
     padded keys / rows are there; key_mask bool [B, Nk]: True = admitted.  scale: default d ** -0.5.  A row without an admitted key, or behind q_lens, gives zeros;
     what stands in keys that are not admitted does not matter.  -> o [B, Nq, H, d], with need_lse also log sum exp of the scores, fp32 [B, H, Nq] (-inf for such rows).
+    need_rest (for the backward, with need_lse): -> (o, lse, rest), rest = what rounding to 16 bits left of o, in the type again (None for float32).
     One row or a few against many keys are split over the keys.  For attention to at most 128 anchors of equal clouds see attention()."""
     a, dev, held = _xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
     o = torch.empty(held[0].shape, dtype=q.dtype, device=dev)
     lse = torch.empty((a.B, a.H, a.Nq), dtype=torch.float32, device=dev) if need_lse else None
-    a.o, a.lse = o.data_ptr(), None if lse is None else lse.data_ptr()
+    rest = torch.empty_like(o) if need_rest and a.type else None
+    a.o, a.rest, a.lse = o.data_ptr(), None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr()
     _xattn_call("ogmm_xattn_fwd", a, dev, 0)
-    return (o, lse) if need_lse else o
+    return (o, lse, rest) if need_rest else (o, lse) if need_lse else o
 
 
-def cross_attention_bwd(q, k, v, o, lse, dout, kv_lens=None, q_lens=None, key_mask=None, scale=None):
-    """Backward of cross_attention(): (dq, dk, dv) from dout = dL/do and the forward's o and lse; the scores are formed again.  Gradients of a key head are summed over
+def cross_attention_bwd(q, k, v, o, lse, dout, kv_lens=None, q_lens=None, key_mask=None, scale=None, rest=None):
+    """Backward of cross_attention(): (dq, dk, dv) from dout = dL/do and the forward's o and lse (and rest); the scores are formed again.  Gradients of a key head are summed over
     the query heads that share it; keys that are not admitted and rows behind q_lens get zeros.  Repeated calls agree bit for bit."""
     a, dev, held = _xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
-    _dev("q", held[0], ("o", o), ("lse", lse), ("dout", dout))
+    _dev("q", held[0], ("o", o), ("lse", lse), ("dout", dout), ("rest", rest))
     if o.shape != held[0].shape or dout.shape != held[0].shape or lse.shape != (a.B, a.H, a.Nq):
         raise _lib.OgmmError("o %s, dout %s and lse %s must be shaped as cross_attention() returns them for q %s" % (tuple(o.shape), tuple(dout.shape), tuple(lse.shape), tuple(q.shape)))
-    if o.dtype != q.dtype:
-        raise _lib.OgmmError("o must be %s, got %s" % (q.dtype, o.dtype))
+    if o.dtype != q.dtype or rest is not None and (rest.dtype != q.dtype or rest.shape != o.shape):
+        raise _lib.OgmmError("o and rest must be %s %s, got %s and %s" % (q.dtype, tuple(o.shape), o.dtype, None if rest is None else (rest.dtype, tuple(rest.shape))))
+    if rest is not None and a.type:
+        rest = _heads(rest.contiguous(), "rest")
+        a.rest = rest.data_ptr()
     dout, o, lse = _heads(dout, "dout", q), _heads(o.contiguous(), "o"), _f32(lse, "lse").contiguous()
     dq = torch.empty(held[0].shape, dtype=q.dtype, device=dev)
     dk, dv = (torch.empty(held[1].shape, dtype=q.dtype, device=dev) for _ in range(2))

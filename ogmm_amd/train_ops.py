@@ -794,20 +794,20 @@ class TrainOps:
 
 # ---------------------------------------------------------------------------------------------- operators of large language models, differentiable
 class _CrossAttention(torch.autograd.Function):
-    """ops.cross_attention with its gradient; saves o and the rows' log sum exp, never the scores"""
+    """ops.cross_attention with its gradient; saves o (16-bit types: and what its rounding left) and the rows' log sum exp, never the scores"""
 
     @staticmethod
     def forward(ctx, q, k, v, kv_lens, q_lens, key_mask, scale):
-        o, lse = ops.cross_attention(q, k, v, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask, scale=scale, need_lse=True)
-        ctx.save_for_backward(q, k, v, o, lse, kv_lens, q_lens, key_mask)
+        o, lse, rest = ops.cross_attention(q, k, v, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask, scale=scale, need_lse=True, need_rest=True)
+        ctx.save_for_backward(q, k, v, o, lse, rest, kv_lens, q_lens, key_mask)
         ctx.scale = scale
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, o, lse, kv_lens, q_lens, key_mask = ctx.saved_tensors
-        dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, g, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask, scale=ctx.scale)
+        q, k, v, o, lse, rest, kv_lens, q_lens, key_mask = ctx.saved_tensors
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, g, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask, scale=ctx.scale, rest=rest)
         return dq, dk, dv, None, None, None, None
 
 

@@ -47,8 +47,8 @@ def attention_case(B, Nq, Nk, H, G, d, dtype, seed, size=1.5):
     return randn(g, B, Nq, H, d, dtype=torch.float32).mul(size).to(dtype), randn(g, B, Nk, H // G, d, dtype=dtype), randn(g, B, Nk, H // G, d, dtype=dtype), randn(g, B, Nq, H, d, dtype=dtype)
 
 
-def reference(q, k, v, do, kv_lens=None, q_lens=None, key_mask=None, scale=None, grads=True):
-    """values and elementwise bounds in 64 bits: {name: (value, bound)}"""
+def reference(q, k, v, do, kv_lens=None, q_lens=None, key_mask=None, scale=None, grads=True, stored=True):
+    """values and elementwise bounds in 64 bits: {name: (value, bound)}; stored = False: o is known to h^2 (its rounding and the rounding of what that left)"""
     B, Nq, H, d = q.shape
     Nk, Hkv = k.shape[1:3]
     G, t = H // Hkv, q.dtype
@@ -82,7 +82,7 @@ def reference(q, k, v, do, kv_lens=None, q_lens=None, key_mask=None, scale=None,
     ds = (d + 8) * U * (Q.abs() @ K.abs().transpose(2, 3).contiguous() * abs(scale)).amax(dim=3, keepdim=True) + 8 * U
     rel_p = 2 * ds + (Nk + 16) * U          # numerator and denominator, the sum over the keys and the rescalings of the running one
     half_p = h if t != torch.float32 else 0.0          # P as an operand of the type's matrix instruction
-    e_o = (rel_p + half_p + Nk * U) * (P @ V.abs()) + a * V.abs().sum(dim=2, keepdim=True) + h * O.abs() + a
+    e_o = (rel_p + half_p + Nk * U) * (P @ V.abs()) + a * V.abs().sum(dim=2, keepdim=True) + (h if stored else h * h) * O.abs() + a
 
     def back(x):
         return x.permute(0, 2, 1, 3)
@@ -132,6 +132,14 @@ def check_attention(q, k, v, do, grads=True, **kw):
             close(x, *want[name], name)
         for x, y in zip(got, ops.cross_attention_bwd(q, k, v, o, lse, do, **kw)):
             assert torch.equal(x, y), "a repeated call differs"
+        # with what the rounding of o left: D is as in fp32
+        o2, lse2, rest = ops.cross_attention(q, k, v, need_lse=True, need_rest=True, **kw)
+        assert torch.equal(o2, o) and torch.equal(lse2, lse) and (rest is None) == (q.dtype == torch.float32)
+        if rest is not None:
+            close(o.double() + rest.double(), *reference(q, k, v, do, grads=False, stored=False, **kw)["o"], "o + rest")
+        want = reference(q, k, v, do, stored=False, **kw)
+        for name, x in zip(("dq", "dk", "dv"), ops.cross_attention_bwd(q, k, v, o, lse, do, rest=rest, **kw)):
+            close(x, *want[name], name + " with the rest")
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
