@@ -52,10 +52,11 @@ __device__ __forceinline__ void mma(f32x16& c, u32x4 a, u32x4 b, float) {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
 }
 
-// A matrix of rows in LDS: ROW bytes and a gap that sets neighbouring rows 16 (or 32) bytes apart in the banks
-template <class T, int DP, int PAD>
+// A matrix of rows in LDS.  The gap sets neighbouring rows sixteen bytes apart in the banks: of 0, 16, 32, 48, 64 bytes it costs the row reads least (181, against 202 cycles for four
+// dependent ones without it, 301 at rows of 256 bytes), and the transposing reads do not mind.
+template <class T, int DP>
 struct Tile {
-    static constexpr int ROW = DP * sizeof(T), PITCH = ROW + PAD, CHUNKS = ROW / 32, DB = DP / 32;
+    static constexpr int ROW = DP * sizeof(T), PITCH = ROW + 16, CHUNKS = ROW / 32, DB = DP / 32;
 
     // row lane % 32 of a block of 32 rows, chunk s of its channels
     static __device__ __forceinline__ u32x4 row_chunk(const char* lds, int row0, int s) {
@@ -114,12 +115,77 @@ __device__ __forceinline__ void as_operand(u32x4 (&y)[sizeof(T) == 4 ? 4 : 2], c
     }
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// the value of lane and of lane ^ 32: their maximum, their sum
+__device__ __forceinline__ float max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // Which of the 64 keys from n0 are admitted, one bit each (the same in every wave)
 __device__ __forceinline__ uint64_t key_bits(const Args& a, int b, int n0, int len) {
+    if (!a.key_mask) return len - n0 >= 64 ? ~uint64_t(0) : len > n0 ? (uint64_t(1) << (len - n0)) - 1 : 0;
     const int n = n0 + (threadIdx.x & 63);
-    return __ballot(n < len && (!a.key_mask || a.key_mask[b * a.mask_b + n]));
+    return __ballot(n < len && a.key_mask[b * a.mask_b + n]);
+}
+
+// Tiles of KT rows on their way to LDS: 256 threads, sixteen bytes each, CPR chunks to a row.  The rows' addresses are a base that every lane shares and 32 bits of a lane's own.
+template <class T, int DP, int KT>
+struct Stage {
+    static constexpr int CPR = DP * static_cast<int>(sizeof(T)) / 16, STEP = 256 / CPR, PASSES = KT / STEP, PITCH = Tile<T, DP>::PITCH;
+    static_assert(PASSES >= 1 && KT % STEP == 0, "shape");
+
+    static __device__ __forceinline__ int chunk() { return threadIdx.x % CPR; }
+    static __device__ __forceinline__ int row() { return threadIdx.x / CPR; }
+    // a chunk behind the head's width reads the row's first, and becomes zeros on the way to LDS
+    static __device__ __forceinline__ uint32_t chunk_offset(int d) { return chunk() * 16 < d * static_cast<int>(sizeof(T)) ? chunk() * 16 : 0; }
+
+    // rows [n0, n0 + KT) of x, `step` bytes apart, of which n are there (rows behind them: the last one)
+    static __device__ __forceinline__ void fetch(u32x4 (&r)[PASSES], const char* __restrict__ x, int64_t step, int n0, int n, uint32_t chunk_off) {
+        const char* tile = x + n0 * step;
+        if (n0 + KT <= n) {
+            const uint32_t mine = row() * static_cast<uint32_t>(step) + chunk_off;
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) r[i] = *reinterpret_cast<const u32x4*>(tile + i * STEP * step + mine);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i)
+                r[i] = *reinterpret_cast<const u32x4*>(tile + (min(row() + i * STEP, n - 1 - n0) * static_cast<uint32_t>(step) + chunk_off));
+        }
+    }
+
+    // A row whose bit is not set becomes zeros: what stands there may be anything, and 0 x NaN is no 0
+    template <int WORDS>
+    static __device__ __forceinline__ void put(char* lds, const u32x4 (&r)[PASSES], const uint64_t (&bits)[WORDS], bool full, int d) {
+        char* p = lds + row() * PITCH + 16 * chunk();
+        if (full && d == DP) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(p + i * STEP * PITCH) = r[i];
+        } else {
+            const bool there = chunk() * 16 < d * static_cast<int>(sizeof(T));
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int n = row() + i * STEP;
+                const bool on = there && (bits[WORDS == 1 ? 0 : n >> 6] >> (n & 63) & 1);
+                *reinterpret_cast<u32x4*>(p + i * STEP * PITCH) = on ? r[i] : u32x4{0, 0, 0, 0};
+            }
+        }
+    }
+};
+
+// A result's start: zeros, or for a lane's sixteen rows 8 (i / 4) + 4 (lane / 32) + i % 4 the values in LDS
+__device__ __forceinline__ f32x16 rows_of(const float* lds) {
+    f32x16 x;
+    lds += 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(lds + 2 * i);
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    }
+    return x;
 }
 
 // a lane's column of a result times f to a row of channels in memory: 16-bit four channels at once, fp32 DB.  rest: what the rounding to 16 bits left, in 16 bits again
@@ -170,65 +236,41 @@ template <class T, int DP, bool KEY_WAVES>
 struct Fwd {
     // keys of a tile: enough products between two barriers, and so little LDS that two workgroups share a CU
     static constexpr int KT = KEY_WAVES ? 128 : sizeof(T) == 4 && DP > 64 ? 32 : 64;
-    using K = Tile<T, DP, 16>;
-    using V = Tile<T, DP, sizeof(T) == 4 ? 16 : 32>;
+    using M = Tile<T, DP>;
     static constexpr int ROWS = KEY_WAVES ? 32 : 128;
-    static constexpr int TILE_BYTES = KT * (K::PITCH + V::PITCH);
+    static constexpr int TILE_BYTES = 2 * KT * M::PITCH + KT * 4;
     // the four waves' sums side by side at the end
     static constexpr int LDS = KEY_WAVES ? std::max(TILE_BYTES, 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8) : TILE_BYTES;
-    static constexpr int CPR = K::ROW / 16, PASSES = KT * CPR / 256;          // chunks of sixteen bytes to a row, rounds of 256 threads to a tile
 };
-
-// rows [n0, n0 + KT) of k or v in registers (rows behind the padded end: some row that is there; channels behind d: zeros)
-template <class T, int CPR, int PASSES>
-__device__ __forceinline__ void fetch(u32x4 (&r)[PASSES], const T* __restrict__ x, int64_t step, int n0, int n, int d) {
-    const int c = threadIdx.x % CPR;
-    const bool there = c * 16 < d * static_cast<int>(sizeof(T));
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int row = min(n0 + static_cast<int>(threadIdx.x) / CPR + i * (256 / CPR), n - 1);
-        r[i] = u32x4{0, 0, 0, 0};
-        if (there) r[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(x + row * step) + 16 * c);
-    }
-}
-
-// ... and from there to LDS; a row that is not admitted becomes zeros: what stands there may be anything, and 0 x NaN is no 0
-template <int PITCH, int CPR, int PASSES, int WORDS>
-__device__ __forceinline__ void put(char* lds, const u32x4 (&r)[PASSES], const uint64_t (&bits)[WORDS], bool full) {
-    const int c = threadIdx.x % CPR;
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int row = static_cast<int>(threadIdx.x) / CPR + i * (256 / CPR);
-        u32x4 v = r[i];
-        if (!full && !(bits[WORDS == 1 ? 0 : row >> 6] >> (row & 63) & 1)) v = u32x4{0, 0, 0, 0};
-        *reinterpret_cast<u32x4*>(lds + row * PITCH + 16 * c) = v;
-    }
-}
 
 template <class T, int DP, bool KEY_WAVES>
 __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) void xattn_fwd_kernel(const Args a) {
     using S = Fwd<T, DP, KEY_WAVES>;
-    using K = typename S::K;
-    using V = typename S::V;
-    constexpr int KT = S::KT, WORDS = KT > 64 ? KT / 64 : 1, BLOCKS = KEY_WAVES ? 1 : KT / 32, DB = K::DB;
+    using M = typename S::M;
+    using St = Stage<T, DP, S::KT>;
+    constexpr int KT = S::KT, WORDS = KT > 64 ? KT / 64 : 1, BLOCKS = KEY_WAVES ? 1 : KT / 32, DB = M::DB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lds_k = lds, *lds_v = lds + KT * K::PITCH;
+    char *lds_k = lds, *lds_v = lds + KT * M::PITCH;
+    float* lds_bias = reinterpret_cast<float*>(lds + 2 * KT * M::PITCH);          // 0, or -inf where a key is not admitted
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int split = item % a.splits, tile = item / a.splits % a.tiles, bh = item / a.splits / a.tiles, hk = bh % a.Hkv, b = bh / a.Hkv;
     const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
-    const T *k = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, *v = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h;
+    const char *k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h);
+    const char *v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h);
+    const int64_t k_step = a.k_n * static_cast<int64_t>(sizeof(T)), v_step = a.v_n * static_cast<int64_t>(sizeof(T));
+    const uint32_t chunk_off = St::chunk_offset(a.d);
     // this lane's query row
     const int row = tile * S::ROWS + (KEY_WAVES ? 0 : wave * 32) + (lane & 31), n = row / a.G, g = row - n * a.G;
     const bool row_there = row < q_rows;
-    u32x4 q[K::CHUNKS];
+    u32x4 q[M::CHUNKS];
     const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;          // (scale = 0: no score, whatever the queries are)
     {
         const char* p = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + b * a.q_b + n * a.q_n + (hk * a.G + g) * a.q_h);
         const uint32_t flip = a.scale < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;          // a negative scale: the queries' signs
 #pragma unroll
-        for (int s = 0; s < K::CHUNKS; ++s) {
+        for (int s = 0; s < M::CHUNKS; ++s) {
             q[s] = u32x4{0, 0, 0, 0};
             if (row_there && a.scale != 0.0f && 32 * s + 16 * (lane >> 5) < a.d * static_cast<int>(sizeof(T))) q[s] = *reinterpret_cast<const u32x4*>(p + 32 * s + 16 * (lane >> 5)) ^ flip;
         }
@@ -237,7 +279,7 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
     const int end = min(key_tiles, (split + 1) * per);
     float m = -INFINITY, l = 0.0f;          // m: of scale S log2(e), the running maximum or up to 8 below it
     f32x16 o[DB] = {};
-    u32x4 rk[S::PASSES], rv[S::PASSES];
+    u32x4 rk[St::PASSES], rv[St::PASSES];
     uint64_t bits[WORDS], next_bits[WORDS];
     auto next = [&](int t) {          // the first tile from t on that has an admitted key
         for (; t < end; ++t) {
@@ -250,43 +292,37 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
     };
     int t = next(split * per);
     if (t < end) {
-        fetch<T, S::CPR>(rk, k, a.k_n, t * KT, a.Nk, a.d);
-        fetch<T, S::CPR>(rv, v, a.v_n, t * KT, a.Nk, a.d);
+        St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
+        St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
     }
     while (t < end) {
         constexpr uint64_t ALL = KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0);
         bool full = true;
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) { bits[w] = next_bits[w]; full &= bits[w] == ALL; }
-        put<K::PITCH, S::CPR>(lds_k, rk, bits, full);
-        put<V::PITCH, S::CPR>(lds_v, rv, bits, full);
+        St::put(lds_k, rk, bits, full, a.d);
+        St::put(lds_v, rv, bits, full, a.d);
+        if (!full && threadIdx.x < KT) lds_bias[threadIdx.x] = bits[WORDS == 1 ? 0 : threadIdx.x >> 6] >> (threadIdx.x & 63) & 1 ? 0.0f : -INFINITY;
         __syncthreads();
         t = next(t + 1);
         if (t < end) {
-            fetch<T, S::CPR>(rk, k, a.k_n, t * KT, a.Nk, a.d);
-            fetch<T, S::CPR>(rv, v, a.v_n, t * KT, a.Nk, a.d);
+            St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
+            St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
         }
         f32x16 s[BLOCKS] = {};
+        if (!full)
+#pragma unroll
+            for (int j = 0; j < BLOCKS; ++j) s[j] = rows_of(lds_bias + (KEY_WAVES ? wave * 32 : 32 * j));
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j)
 #pragma unroll
-            for (int u = 0; u < K::CHUNKS; ++u) mma(s[j], K::row_chunk(lds_k, KEY_WAVES ? wave * 32 : 32 * j, u), q[u], T());
-        if (!full) {
-#pragma unroll
-            for (int j = 0; j < BLOCKS; ++j) {
-                const int key0 = KEY_WAVES ? wave * 32 : 32 * j;
-                const uint32_t mine = static_cast<uint32_t>(bits[WORDS == 1 ? 0 : key0 >> 6] >> (key0 & 63)) >> (4 * (lane >> 5));
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(mine >> (8 * (i / 4) + i % 4) & 1)) s[j][i] = -INFINITY;
-            }
-        }
+            for (int u = 0; u < M::CHUNKS; ++u) mma(s[j], M::row_chunk(lds_k, KEY_WAVES ? wave * 32 : 32 * j, u), q[u], T());
         float top = s[0][0];
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
-        top = fmaxf(top, other_half(top)) * c;
+        top = max_halves(top) * c;
         // The sums are brought to a new maximum only where it rose by more than 2^8: weights up to 2^8 keep their relative precision in every type
         if (__ballot(top > m + 8.0f)) {
             const float up = fmaxf(m, top), f = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - up);
@@ -300,20 +336,19 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
         const float shift = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
-            float part = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, -shift));
-                part += s[j][i];
-            }
-            l += part;
+            for (int i = 0; i < 16; ++i) s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, -shift));
             u32x4 p[sizeof(T) == 4 ? 4 : 2];
             as_operand<T>(p, s[j]);
-            V::mul_t(o, lds_v, KEY_WAVES ? wave * 32 : 32 * j, p);
+            float part = 0.0f;          // (of the weights as they are in 32 bits: lse is what the backward's weights are made of)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) part += s[j][i];
+            l += part;
+            M::mul_t(o, lds_v, KEY_WAVES ? wave * 32 : 32 * j, p);
         }
         __syncthreads();
     }
-    l += other_half(l);
+    l = add_halves(l);
     if (!row_there) {          // (behind q_lens: it has looked at keys with the zeros it was given)
         m = -INFINITY;
         l = 0.0f;
@@ -332,7 +367,7 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sums[(wave * 32 + (lane & 31)) * (DP + 4) + K::channel(db, i)] = o[db][i] * f;
+            for (int i = 0; i < 16; ++i) sums[(wave * 32 + (lane & 31)) * (DP + 4) + M::channel(db, i)] = o[db][i] * f;
         __syncthreads();
         const int r = threadIdx.x >> 3;          // eight threads to a row
         const int out_row = tile * 32 + r;
@@ -361,11 +396,11 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
         if (row >= a.rows) return;
         if (a.splits > 1) {
             if (lane < 32) reinterpret_cast<float2*>(a.part_ml)[static_cast<int64_t>(item) * S::ROWS + wave * 32 + lane] = make_float2(m, l);
-            store_part<K>(a.part + (static_cast<int64_t>(item) * S::ROWS + wave * 32 + (lane & 31)) * a.d, o, 1.0f, a.d);
+            store_part<M>(a.part + (static_cast<int64_t>(item) * S::ROWS + wave * 32 + (lane & 31)) * a.d, o, 1.0f, a.d);
             return;
         }
         const int64_t out = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
-        store_column<T, K>(static_cast<T*>(a.o) + out, a.rest ? static_cast<T*>(a.rest) + out : nullptr, o, l > 0.0f ? 1.0f / l : l, a.d);
+        store_column<T, M>(static_cast<T*>(a.o) + out, a.rest ? static_cast<T*>(a.rest) + out : nullptr, o, l > 0.0f ? 1.0f / l : l, a.d);
         if (a.lse && lane < 32) a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
     }
 }
@@ -473,8 +508,7 @@ __device__ __forceinline__ float gradient_scale(const BwdArgs& a, int bh) {
 template <class T, int DP>
 struct Bwd {
     static constexpr int KT = sizeof(T) == 4 && DP > 64 ? 32 : 64;          // keys (dq) or rows (dk, dv) of a tile
-    using M = Tile<T, DP, sizeof(T) == 4 ? 16 : 32>;
-    static constexpr int CPR = M::ROW / 16, PASSES = KT * CPR / 256;
+    using M = Tile<T, DP>;
     static constexpr int LDS = 2 * KT * M::PITCH + 2 * KT * 4;
 };
 
@@ -482,18 +516,24 @@ template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
     using M = typename S::M;
+    using St = Stage<T, DP, S::KT>;
     constexpr int KT = S::KT, BLOCKS = KT / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char *lds_k = lds, *lds_v = lds + KT * M::PITCH;
+    float* lds_bias = reinterpret_cast<float*>(lds + 2 * KT * M::PITCH);
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int split = item % a.row_splits, tile = item / a.row_splits % a.row_tiles, bh = item / a.row_splits / a.row_tiles, hk = bh % a.Hkv, b = bh / a.Hkv;
     const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
-    const T *k = static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, *v = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h;
+    const char *k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h);
+    const char *v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h);
+    const int64_t k_step = a.k_n * static_cast<int64_t>(sizeof(T)), v_step = a.v_n * static_cast<int64_t>(sizeof(T));
+    const uint32_t chunk_off = St::chunk_offset(a.d);
     const int row = tile * 128 + wave * 32 + (lane & 31);
     const bool row_there = row < q_rows;
-    const float c = a.scale * LOG2E, up = gradient_scale<T>(a, bh);
+    // (a negative scale turns the queries' signs, so that -inf is below every score; scale = 0: no score)
+    const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E, up = gradient_scale<T>(a, bh);
     u32x4 q[M::CHUNKS], go[M::CHUNKS];
     float lse2 = INFINITY, delta = 0.0f;
     {
@@ -501,19 +541,20 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
         if (row_there) { lse2 = a.lse2[at]; delta = a.delta[at]; }
         const char* pq = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + row_offset(a, row, b, hk, a.q_b, a.q_n, a.q_h));
         const char* pg = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + row_offset(a, row, b, hk, a.do_b, a.do_n, a.do_h));
+        const uint32_t flip = a.scale < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
         for (int s = 0; s < M::CHUNKS; ++s) {
             const int at = 32 * s + 16 * (lane >> 5);
             q[s] = go[s] = u32x4{0, 0, 0, 0};
             if (row_there && at < a.d * static_cast<int>(sizeof(T))) {
-                q[s] = *reinterpret_cast<const u32x4*>(pq + at);
+                if (a.scale != 0.0f) q[s] = *reinterpret_cast<const u32x4*>(pq + at) ^ flip;
                 go[s] = *reinterpret_cast<const u32x4*>(pg + at);
             }
         }
     }
     const int tiles = tile * 128 < q_rows ? (len + KT - 1) / KT : 0, per = (tiles + a.row_splits - 1) / a.row_splits, end = min(tiles, (split + 1) * per);
     f32x16 dq[M::DB] = {};
-    u32x4 rk[S::PASSES], rv[S::PASSES];
+    u32x4 rk[St::PASSES], rv[St::PASSES];
     uint64_t bits[1], next_bits = 0;
     auto next = [&](int t) {
         for (; t < end; ++t)
@@ -522,34 +563,31 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
     };
     int t = next(split * per);
     if (t < end) {
-        fetch<T, S::CPR>(rk, k, a.k_n, t * KT, a.Nk, a.d);
-        fetch<T, S::CPR>(rv, v, a.v_n, t * KT, a.Nk, a.d);
+        St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
+        St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
     }
     while (t < end) {
         bits[0] = next_bits;
         const bool full = bits[0] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
-        put<M::PITCH, S::CPR>(lds_k, rk, bits, full);
-        put<M::PITCH, S::CPR>(lds_v, rv, bits, full);
+        St::put(lds_k, rk, bits, full, a.d);
+        St::put(lds_v, rv, bits, full, a.d);
+        if (!full && threadIdx.x < KT) lds_bias[threadIdx.x] = bits[0] >> threadIdx.x & 1 ? 0.0f : -INFINITY;
         __syncthreads();
         t = next(t + 1);
         if (t < end) {
-            fetch<T, S::CPR>(rk, k, a.k_n, t * KT, a.Nk, a.d);
-            fetch<T, S::CPR>(rv, v, a.v_n, t * KT, a.Nk, a.d);
+            St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
+            St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
         }
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
             f32x16 s = {}, dp = {};
+            if (!full) s = rows_of(lds_bias + 32 * j);          // (a key that is not admitted: weight 0, and with its zeros for v a finite dP)
 #pragma unroll
             for (int u = 0; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_k, 32 * j, u), q[u], T());
 #pragma unroll
             for (int u = 0; u < M::CHUNKS; ++u) mma(dp, M::row_chunk(lds_v, 32 * j, u), go[u], T());
-            const uint32_t mine = static_cast<uint32_t>(bits[0] >> (32 * j)) >> (4 * (lane >> 5));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2));
-                s[i] = p * (dp[i] - delta) * up;
-                if (!full && !(mine >> (8 * (i / 4) + i % 4) & 1)) s[i] = 0.0f;
-            }
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * (dp[i] - delta) * up;
             u32x4 ds[sizeof(T) == 4 ? 4 : 2];
             as_operand<T>(ds, s);
             M::mul_t(dq, lds_k, 32 * j, ds);
@@ -564,23 +602,11 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
     else store_column<T, M>(static_cast<T*>(a.dq) + at, nullptr, dq, f, a.d);
 }
 
-// rows [r0, r0 + KT) of q or dout
-template <class T, int CPR, int PASSES>
-__device__ __forceinline__ void fetch_rows(u32x4 (&x)[PASSES], const Args& a, const void* p, int64_t sb, int64_t sn, int64_t sh, int r0, int b, int hk) {
-    const int c = threadIdx.x % CPR;
-    const bool there = c * 16 < a.d * static_cast<int>(sizeof(T));
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int r = min(r0 + static_cast<int>(threadIdx.x) / CPR + i * (256 / CPR), a.rows - 1);
-        x[i] = u32x4{0, 0, 0, 0};
-        if (there) x[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(static_cast<const T*>(p) + row_offset(a, r, b, hk, sb, sn, sh)) + 16 * c);
-    }
-}
-
 template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
     using M = typename S::M;
+    using St = Stage<T, DP, S::KT>;
     constexpr int QT = S::KT, BLOCKS = QT / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char *lds_q = lds, *lds_g = lds + QT * M::PITCH;
@@ -611,12 +637,38 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
     }
     const int tiles = any ? (q_rows + QT - 1) / QT : 0, per = (tiles + a.key_splits - 1) / a.key_splits, end = min(tiles, (split + 1) * per);
     f32x16 dk[M::DB] = {}, dv[M::DB] = {};
-    u32x4 rq[S::PASSES], rg[S::PASSES];
+    u32x4 rq[St::PASSES], rg[St::PASSES];
     float r_stat = 0.0f;          // threads 0 .. QT: a row's lse, QT .. 2 QT: its delta
+    const char *q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + b * a.q_b + hk * a.G * a.q_h);
+    const char *go = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + b * a.do_b + hk * a.G * a.do_h);
+    const int64_t q_step = a.q_n * static_cast<int64_t>(sizeof(T)), go_step = a.do_n * static_cast<int64_t>(sizeof(T));
+    const uint32_t q_head = static_cast<uint32_t>(a.q_h * sizeof(T)), go_head = static_cast<uint32_t>(a.do_h * sizeof(T)), chunk_off = St::chunk_offset(a.d);
+    // a tile holds whole rows of all G heads: a lane's place in it is the same for every tile
+    const bool whole = QT % a.G == 0;
+    uint32_t at_q[St::PASSES], at_go[St::PASSES];
+#pragma unroll
+    for (int i = 0; i < St::PASSES; ++i) {
+        const int r = St::row() + i * St::STEP, n = r / a.G, g = r - n * a.G;
+        at_q[i] = n * static_cast<uint32_t>(q_step) + g * q_head + chunk_off;
+        at_go[i] = n * static_cast<uint32_t>(go_step) + g * go_head + chunk_off;
+    }
     auto fetch_tile = [&](int t) {
-        fetch_rows<T, S::CPR>(rq, a, a.q, a.q_b, a.q_n, a.q_h, t * QT, b, hk);
-        fetch_rows<T, S::CPR>(rg, a, a.dout, a.do_b, a.do_n, a.do_h, t * QT, b, hk);
-        const int r = t * QT + threadIdx.x % QT;
+        const int r0 = t * QT;
+        if (whole && r0 + QT <= a.rows) {
+            const char *tq = q + r0 / a.G * q_step, *tg = go + r0 / a.G * go_step;
+#pragma unroll
+            for (int i = 0; i < St::PASSES; ++i) rq[i] = *reinterpret_cast<const u32x4*>(tq + at_q[i]);
+#pragma unroll
+            for (int i = 0; i < St::PASSES; ++i) rg[i] = *reinterpret_cast<const u32x4*>(tg + at_go[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < St::PASSES; ++i) {
+                const int r = min(r0 + St::row() + i * St::STEP, a.rows - 1), n = r / a.G, g = r - n * a.G;
+                rq[i] = *reinterpret_cast<const u32x4*>(q + n * q_step + (g * q_head + chunk_off));
+                rg[i] = *reinterpret_cast<const u32x4*>(go + n * go_step + (g * go_head + chunk_off));
+            }
+        }
+        const int r = r0 + threadIdx.x % QT;
         if (threadIdx.x < 2 * QT) r_stat = r < q_rows ? (threadIdx.x < QT ? a.lse2 : a.delta)[static_cast<int64_t>(bh) * a.rows + r] : threadIdx.x < QT ? INFINITY : 0.0f;
     };
     int t = split * per;
@@ -625,27 +677,23 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
         const int left = q_rows - t * QT;
         const uint64_t bits[1] = {left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1};          // rows behind q_lens become zeros
         const bool full = left >= QT;
-        put<M::PITCH, S::CPR>(lds_q, rq, bits, full);
-        put<M::PITCH, S::CPR>(lds_g, rg, bits, full);
-        if (threadIdx.x < 2 * QT) lds_lse[threadIdx.x] = r_stat;
+        St::put(lds_q, rq, bits, full, a.d);
+        St::put(lds_g, rg, bits, full, a.d);
+        if (threadIdx.x < 2 * QT) lds_lse[threadIdx.x] = -r_stat;
         __syncthreads();
         if (t + 1 < end) fetch_tile(t + 1);
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
-            f32x16 s = {}, dp = {};
+            f32x16 s = {}, dp = rows_of(lds_delta + 32 * j);          // dP - delta from the start
+            const f32x16 l = rows_of(lds_lse + 32 * j);
 #pragma unroll
             for (int u = 0; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_q, 32 * j, u), k[u], T());
 #pragma unroll
             for (int u = 0; u < M::CHUNKS; ++u) mma(dp, M::row_chunk(lds_g, 32 * j, u), v[u], T());
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int r = 32 * j + 2 * i + 4 * (lane >> 5);          // result row 8 (i / 4) + 4 (lane / 32) + i % 4
-                const float4 l4 = *reinterpret_cast<const float4*>(lds_lse + r), d4 = *reinterpret_cast<const float4*>(lds_delta + r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[i + e] = __builtin_amdgcn_exp2f(fmaf(s[i + e], c, -(&l4.x)[e]));
-                    dp[i + e] = s[i + e] * (dp[i + e] - (&d4.x)[e]) * up;
-                }
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, l[i]));
+                dp[i] = s[i] * dp[i] * up;
             }
             u32x4 y[sizeof(T) == 4 ? 4 : 2];
             as_operand<T>(y, s);
@@ -700,6 +748,19 @@ int with_width(int d, F&& f) {
     return f(integral_constant<int, 128>());
 }
 
+// Into how many parts the other sequence's n rows are cut, for `tiles` workgroups on a part that holds `slots` of them at once: parts of 256 rows at least, as many as shorten
+// the sum of the rounds by more than a part costs in writing and joining (taken as 1/16 of a round of it).
+int parts_for(int64_t tiles, int64_t n, int64_t slots) {
+    int best = 1;
+    double least = 1e30;
+    for (int64_t s = 1; s <= std::min<int64_t>((n + 255) / 256, 512); ++s) {
+        const double t = static_cast<double>((tiles * s + slots - 1) / slots) / s + (s > 1 ? s * tiles / (16.0 * slots) : 0.0);
+        if (t < least * 0.999) { least = t; best = static_cast<int>(s); }
+        if (tiles * s > 4 * slots) break;
+    }
+    return best;
+}
+
 // Up to 32 query rows of a key head (single tokens): one row tile, and the four waves of its workgroup take different keys.
 bool few_rows(const ogmm_xattn* a) { return static_cast<int64_t>(a->Nq) * (a->H / a->Hkv) <= 32; }
 
@@ -718,9 +779,9 @@ Args forward_args(const ogmm_xattn* x, float* ws) {
     a.rows = a.Nq * a.G;
     const int tile_rows = few_rows(x) ? 32 : 128;
     a.tiles = (a.rows + tile_rows - 1) / tile_rows;
-    // Where the row tiles alone do not give every CU two workgroups, the keys are cut, into parts of at least 256
+    // Where the row tiles alone do not give every CU two workgroups, the keys are cut
     const int64_t base = static_cast<int64_t>(a.B) * a.Hkv * a.tiles;
-    a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(base, 1), (a.Nk + 255) / 256)));
+    a.splits = parts_for(base, a.Nk, 512);
     a.items = static_cast<uint32_t>(base * a.splits);
     a.part_ml = ws;
     a.part = ws ? ws + static_cast<int64_t>(a.items) * tile_rows * 2 : nullptr;
@@ -753,10 +814,9 @@ BwdArgs backward_args(const ogmm_xattn* x, float* ws, int64_t* floats) {
     a.row_tiles = (a.rows + 127) / 128;
     a.key_tiles = (a.Nk + 127) / 128;
     a.delta_blocks = (a.rows + 63) / 64;
-    // as in the forward: parts where the tiles alone leave CUs without work, of 256 keys or rows at least
-    auto parts = [&](int64_t tiles, int64_t n) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), (n + 255) / 256))); };
-    a.row_splits = parts(heads * a.row_tiles, a.Nk);
-    a.key_splits = parts(heads * a.key_tiles, a.rows);
+    const bool wide = a.d * (a.type == OGMM_F32 ? 2 : 1) > 64;          // (the kernel that owns keys has a CU to itself then)
+    a.row_splits = parts_for(heads * a.row_tiles, a.Nk, 512);
+    a.key_splits = parts_for(heads * a.key_tiles, a.rows, wide ? 256 : 512);
     int64_t n = 0;
     auto take = [&](int64_t count) {
         float* at = ws ? ws + n : nullptr;
@@ -800,6 +860,11 @@ int launch_bwd(BwdArgs a, hipStream_t stream) {
     return check_launch("ogmm_xattn_bwd");
 }
 
+bool steps_fit(const ogmm_xattn* a, int64_t n, int64_t h) {
+    const int64_t e = a->type == OGMM_F32 ? 4 : 2, most = int64_t(1) << 25;
+    return n >= 0 && h >= 0 && n * e < most && h * e < most && 64 * n * e + a->H / a->Hkv * h * e < int64_t(1) << 32;
+}
+
 int check(const char* who, const ogmm_xattn* a) {
     OGMM_REQUIRE(a, "%s: missing argument", who);
     OGMM_REQUIRE(a->B >= 0 && a->Nq >= 0 && a->Nk >= 0 && a->H >= 1 && a->Hkv >= 1, "%s: B = %d, Nq = %d, Nk = %d, H = %d, Hkv = %d", who, a->B, a->Nq, a->Nk, a->H, a->Hkv);
@@ -809,6 +874,8 @@ int check(const char* who, const ogmm_xattn* a) {
     const int64_t e = a->type == OGMM_F32 ? 4 : 2;
     const int64_t strides[] = {a->q_b, a->q_n, a->q_h, a->k_b, a->k_n, a->k_h, a->v_b, a->v_n, a->v_h};
     for (int64_t s : strides) OGMM_REQUIRE(s * e % 16 == 0, "%s: a stride of %lld elements is not a multiple of 16 bytes", who, static_cast<long long>(s));
+    // (the places of 64 rows and of all heads of a row stay within 32 bits)
+    OGMM_REQUIRE(steps_fit(a, a->q_n, a->q_h) && steps_fit(a, a->k_n, 0) && steps_fit(a, a->v_n, 0), "%s: rows or heads are too far apart (32 MB and more)", who);
     OGMM_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->rest), "%s: addresses must be multiples of 16 bytes", who);
     OGMM_REQUIRE(isfinite(a->scale), "%s: scale must be finite", who);
     // (a workgroup takes several rows, so this keeps every grid below 2^31 workgroups and a row's number within 32 bits)
@@ -850,7 +917,8 @@ extern "C" int ogmm_xattn_fwd(const ogmm_xattn* x, void* stream) {
 extern "C" int ogmm_xattn_bwd(const ogmm_xattn* a, void* stream) {
     if (check("ogmm_xattn_bwd", a)) return 1;
     const int64_t e = a->type == OGMM_F32 ? 4 : 2;
-    OGMM_REQUIRE(a->do_b * e % 16 == 0 && a->do_n * e % 16 == 0 && a->do_h * e % 16 == 0 && aligned16(a->dout), "ogmm_xattn_bwd: dout's address and strides must be multiples of 16 bytes");
+    OGMM_REQUIRE(a->do_b * e % 16 == 0 && a->do_n * e % 16 == 0 && a->do_h * e % 16 == 0 && aligned16(a->dout) && steps_fit(a, a->do_n, a->do_h),
+                 "ogmm_xattn_bwd: dout's address and strides must be multiples of 16 bytes, rows and heads less than 32 MB apart");
     OGMM_REQUIRE(aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv), "ogmm_xattn_bwd: addresses must be multiples of 16 bytes");
     const int64_t rows = static_cast<int64_t>(a->B) * a->H * a->Nq, keys = static_cast<int64_t>(a->B) * a->Hkv * a->Nk;
     OGMM_REQUIRE(!rows || (a->dout && a->lse && a->dq), "ogmm_xattn_bwd: missing argument");

@@ -1206,7 +1206,7 @@ def _heads(t, name, like=None):
         raise _lib.OgmmError("%s must be %s, got %s" % (name, like.dtype, t.dtype))
     b, n, h, one = t.stride()
     step = 16 // t.element_size()
-    if (one != 1 and t.shape[3] != 1) or (b | n | h) % step or t.data_ptr() % 16:
+    if (one != 1 and t.shape[3] != 1) or (b | n | h) % step or t.data_ptr() % 16 or max(n, h) * t.element_size() >= 1 << 25:
         t = t.contiguous()
         if t.data_ptr() % 16:          # (contiguous already, at an odd address)
             t = t.clone()

@@ -32,7 +32,7 @@ def xattn(**kw):
 
 BAD_ATTENTION = [dict(B=-1), dict(Nq=-1), dict(Nk=-5), dict(H=0), dict(Hkv=0), dict(H=3), dict(d=0), dict(d=4), dict(d=60), dict(d=136), dict(type=3), dict(type=-1),
                  dict(q_n=255), dict(k_h=65), dict(v_b=4), dict(q=4098), dict(k=4104), dict(v=4097), dict(o=4104), dict(q=None), dict(k=None), dict(v=None), dict(o=None),
-                 dict(scale=math.nan), dict(scale=math.inf), dict(B=1 << 20, H=1 << 16, Hkv=1, Nq=1 << 20)]
+                 dict(k_n=1 << 24), dict(q_h=1 << 24), dict(q_n=-256), dict(scale=math.nan), dict(scale=math.inf), dict(B=1 << 20, H=1 << 16, Hkv=1, Nq=1 << 20)]
 
 
 @pytest.mark.parametrize("kw", BAD_ATTENTION, ids=str)
