@@ -165,12 +165,13 @@ struct Stage {
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) *reinterpret_cast<u32x4*>(p + i * STEP * PITCH) = r[i];
         } else {
-            const bool there = chunk() * 16 < d * static_cast<int>(sizeof(T));
+            const uint32_t there = chunk() * 16 < d * static_cast<int>(sizeof(T)) ? 1 : 0;
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
                 const int n = row() + i * STEP;
-                const bool on = there && (bits[WORDS == 1 ? 0 : n >> 6] >> (n & 63) & 1);
-                *reinterpret_cast<u32x4*>(p + i * STEP * PITCH) = on ? r[i] : u32x4{0, 0, 0, 0};
+                const uint64_t word = bits[WORDS == 1 ? 0 : n >> 6];
+                const uint32_t keep = -(static_cast<uint32_t>(word >> (n & 63)) & there);
+                *reinterpret_cast<u32x4*>(p + i * STEP * PITCH) = r[i] & keep;
             }
         }
     }
@@ -239,8 +240,9 @@ struct Fwd {
     using M = Tile<T, DP>;
     static constexpr int ROWS = KEY_WAVES ? 32 : 128;
     static constexpr int TILE_BYTES = 2 * KT * M::PITCH + KT * 4;
-    // the four waves' sums side by side at the end
-    static constexpr int LDS = KEY_WAVES ? std::max(TILE_BYTES, 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8) : TILE_BYTES;
+    // Query waves: two tiles, so that one is written while the other is read, and there is one barrier to a tile; key waves: one, and the four waves' sums side by side at the end
+    static constexpr int BUFFERS = KEY_WAVES ? 1 : 2;
+    static constexpr int LDS = KEY_WAVES ? std::max(TILE_BYTES, 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8) : BUFFERS * TILE_BYTES;
 };
 
 template <class T, int DP, bool KEY_WAVES>
@@ -250,8 +252,9 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
     using St = Stage<T, DP, S::KT>;
     constexpr int KT = S::KT, WORDS = KT > 64 ? KT / 64 : 1, BLOCKS = KEY_WAVES ? 1 : KT / 32, DB = M::DB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lds_k = lds, *lds_v = lds + KT * M::PITCH;
-    float* lds_bias = reinterpret_cast<float*>(lds + 2 * KT * M::PITCH);          // 0, or -inf where a key is not admitted
+    // a tile: keys, values, and 0 or -inf for a key that is not admitted
+    uint32_t buffer = 0;          // where in LDS the tile that is read begins; the other: OTHER - buffer
+    constexpr uint32_t OTHER = (S::BUFFERS - 1) * S::TILE_BYTES;
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
     float m = -INFINITY, l = 0.0f;          // m: of scale S log2(e), the running maximum or up to 8 below it
     f32x16 o[DB] = {};
     u32x4 rk[St::PASSES], rv[St::PASSES];
-    uint64_t bits[WORDS], next_bits[WORDS];
+    uint64_t next_bits[WORDS];
     auto next = [&](int t) {          // the first tile from t on that has an admitted key
         for (; t < end; ++t) {
             uint64_t any = 0;
@@ -290,33 +293,44 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
         }
         return t;
     };
-    int t = next(split * per);
-    if (t < end) {
+    auto fetch = [&](int t) {
         St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
         St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
-    }
-    while (t < end) {
-        constexpr uint64_t ALL = KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0);
-        bool full = true;
+    };
+    bool full = true;
+    auto put = [&](char* to) {          // (what next() found out about the tile goes with it)
+        full = true;
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w) { bits[w] = next_bits[w]; full &= bits[w] == ALL; }
-        St::put(lds_k, rk, bits, full, a.d);
-        St::put(lds_v, rv, bits, full, a.d);
-        if (!full && threadIdx.x < KT) lds_bias[threadIdx.x] = bits[WORDS == 1 ? 0 : threadIdx.x >> 6] >> (threadIdx.x & 63) & 1 ? 0.0f : -INFINITY;
+        for (int w = 0; w < WORDS; ++w) full &= next_bits[w] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
+        St::put(to, rk, next_bits, full, a.d);
+        St::put(to + KT * M::PITCH, rv, next_bits, full, a.d);
+        if (!full && threadIdx.x < KT)
+            reinterpret_cast<float*>(to + 2 * KT * M::PITCH)[threadIdx.x] = next_bits[WORDS == 1 ? 0 : threadIdx.x >> 6] >> (threadIdx.x & 63) & 1 ? 0.0f : -INFINITY;
+    };
+    int t = next(split * per);
+    bool more = t < end;
+    if (more) {
+        fetch(t);
+        put(lds);
         __syncthreads();
+    }
+    while (more) {
+        const bool all = full;
+        const char *lds_k = lds + buffer, *lds_v = lds_k + KT * M::PITCH;
+        const float* lds_bias = reinterpret_cast<const float*>(lds_k + 2 * KT * M::PITCH);
         t = next(t + 1);
-        if (t < end) {
-            St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
-            St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
+        more = t < end;
+        if (more) fetch(t);
+        f32x16 s[BLOCKS];
+#pragma unroll
+        for (int j = 0; j < BLOCKS; ++j) {
+            const int key0 = KEY_WAVES ? wave * 32 : 32 * j;
+            s[j] = f32x16{};
+            if (all) mma(s[j], M::row_chunk(lds_k, key0, 0), q[0], T());
+            else mma(s[j] = rows_of(lds_bias + key0), M::row_chunk(lds_k, key0, 0), q[0], T());
+#pragma unroll
+            for (int u = 1; u < M::CHUNKS; ++u) mma(s[j], M::row_chunk(lds_k, key0, u), q[u], T());
         }
-        f32x16 s[BLOCKS] = {};
-        if (!full)
-#pragma unroll
-            for (int j = 0; j < BLOCKS; ++j) s[j] = rows_of(lds_bias + (KEY_WAVES ? wave * 32 : 32 * j));
-#pragma unroll
-        for (int j = 0; j < BLOCKS; ++j)
-#pragma unroll
-            for (int u = 0; u < M::CHUNKS; ++u) mma(s[j], M::row_chunk(lds_k, KEY_WAVES ? wave * 32 : 32 * j, u), q[u], T());
         float top = s[0][0];
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j)
@@ -346,7 +360,10 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
             l += part;
             M::mul_t(o, lds_v, KEY_WAVES ? wave * 32 : 32 * j, p);
         }
-        __syncthreads();
+        if constexpr (S::BUFFERS == 1) __syncthreads();
+        if (more) put(lds + (OTHER - buffer));
+        if (more || KEY_WAVES) __syncthreads();
+        buffer = OTHER - buffer;
     }
     l = add_halves(l);
     if (!row_there) {          // (behind q_lens: it has looked at keys with the zeros it was given)
@@ -509,7 +526,7 @@ template <class T, int DP>
 struct Bwd {
     static constexpr int KT = sizeof(T) == 4 && DP > 64 ? 32 : 64;          // keys (dq) or rows (dk, dv) of a tile
     using M = Tile<T, DP>;
-    static constexpr int LDS = 2 * KT * M::PITCH + 2 * KT * 4;
+    static constexpr int TILE_BYTES = 2 * KT * M::PITCH + 2 * KT * 4, LDS = 2 * TILE_BYTES;
 };
 
 template <class T, int DP>
@@ -519,8 +536,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
     using St = Stage<T, DP, S::KT>;
     constexpr int KT = S::KT, BLOCKS = KT / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lds_k = lds, *lds_v = lds + KT * M::PITCH;
-    float* lds_bias = reinterpret_cast<float*>(lds + 2 * KT * M::PITCH);
+    uint32_t buffer = 0;          // where in LDS the tile that is read begins; the other: OTHER - buffer
+    constexpr uint32_t OTHER = S::TILE_BYTES;
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -555,44 +572,60 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
     const int tiles = tile * 128 < q_rows ? (len + KT - 1) / KT : 0, per = (tiles + a.row_splits - 1) / a.row_splits, end = min(tiles, (split + 1) * per);
     f32x16 dq[M::DB] = {};
     u32x4 rk[St::PASSES], rv[St::PASSES];
-    uint64_t bits[1], next_bits = 0;
+    uint64_t next_bits[1] = {0};
     auto next = [&](int t) {
         for (; t < end; ++t)
-            if ((next_bits = key_bits(a, b, t * KT, min(len, (t + 1) * KT)))) break;
+            if ((next_bits[0] = key_bits(a, b, t * KT, min(len, (t + 1) * KT)))) break;
         return t;
     };
-    int t = next(split * per);
-    if (t < end) {
+    auto fetch = [&](int t) {
         St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
         St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
-    }
-    while (t < end) {
-        bits[0] = next_bits;
-        const bool full = bits[0] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
-        St::put(lds_k, rk, bits, full, a.d);
-        St::put(lds_v, rv, bits, full, a.d);
-        if (!full && threadIdx.x < KT) lds_bias[threadIdx.x] = bits[0] >> threadIdx.x & 1 ? 0.0f : -INFINITY;
+    };
+    bool full = true;
+    auto put = [&](char* to) {
+        full = next_bits[0] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
+        St::put(to, rk, next_bits, full, a.d);
+        St::put(to + KT * M::PITCH, rv, next_bits, full, a.d);
+        if (!full && threadIdx.x < KT) reinterpret_cast<float*>(to + 2 * KT * M::PITCH)[threadIdx.x] = next_bits[0] >> threadIdx.x & 1 ? 0.0f : -INFINITY;
+    };
+    f32x16 start;          // dP - delta from the start
+#pragma unroll
+    for (int i = 0; i < 16; ++i) start[i] = -delta;
+    int t = next(split * per);
+    bool more = t < end;
+    if (more) {
+        fetch(t);
+        put(lds);
         __syncthreads();
+    }
+    while (more) {
+        const bool all = full;
+        const char *lds_k = lds + buffer, *lds_v = lds_k + KT * M::PITCH;
+        const float* lds_bias = reinterpret_cast<const float*>(lds_k + 2 * KT * M::PITCH);
         t = next(t + 1);
-        if (t < end) {
-            St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
-            St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
-        }
+        more = t < end;
+        if (more) fetch(t);
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
-            f32x16 s = {}, dp = {};
-            if (!full) s = rows_of(lds_bias + 32 * j);          // (a key that is not admitted: weight 0, and with its zeros for v a finite dP)
+            f32x16 s = {}, dp = start;
+            if (all) mma(s, M::row_chunk(lds_k, 32 * j, 0), q[0], T());
+            else mma(s = rows_of(lds_bias + 32 * j), M::row_chunk(lds_k, 32 * j, 0), q[0], T());          // (a key that is not admitted: weight 0, and with its zeros for v a finite dP)
 #pragma unroll
-            for (int u = 0; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_k, 32 * j, u), q[u], T());
+            for (int u = 1; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_k, 32 * j, u), q[u], T());
 #pragma unroll
             for (int u = 0; u < M::CHUNKS; ++u) mma(dp, M::row_chunk(lds_v, 32 * j, u), go[u], T());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * (dp[i] - delta) * up;
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * dp[i] * up;
             u32x4 ds[sizeof(T) == 4 ? 4 : 2];
             as_operand<T>(ds, s);
             M::mul_t(dq, lds_k, 32 * j, ds);
         }
-        __syncthreads();
+        if (more) {
+            put(lds + (OTHER - buffer));
+            __syncthreads();
+        }
+        buffer = OTHER - buffer;
     }
     if (row >= a.rows) return;
     const int n = row / a.G, g = row - n * a.G;
@@ -609,8 +642,9 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
     using St = Stage<T, DP, S::KT>;
     constexpr int QT = S::KT, BLOCKS = QT / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char *lds_q = lds, *lds_g = lds + QT * M::PITCH;
-    float *lds_lse = reinterpret_cast<float*>(lds + 2 * QT * M::PITCH), *lds_delta = lds_lse + QT;
+    // a tile: rows of q, of dout, their -lse, their -delta
+    uint32_t buffer = 0;
+    constexpr uint32_t OTHER = S::TILE_BYTES;
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -671,16 +705,22 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
         const int r = r0 + threadIdx.x % QT;
         if (threadIdx.x < 2 * QT) r_stat = r < q_rows ? (threadIdx.x < QT ? a.lse2 : a.delta)[static_cast<int64_t>(bh) * a.rows + r] : threadIdx.x < QT ? INFINITY : 0.0f;
     };
-    int t = split * per;
-    if (t < end) fetch_tile(t);
-    for (; t < end; ++t) {
+    auto put = [&](char* to, int t) {
         const int left = q_rows - t * QT;
         const uint64_t bits[1] = {left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1};          // rows behind q_lens become zeros
-        const bool full = left >= QT;
-        St::put(lds_q, rq, bits, full, a.d);
-        St::put(lds_g, rg, bits, full, a.d);
-        if (threadIdx.x < 2 * QT) lds_lse[threadIdx.x] = -r_stat;
+        St::put(to, rq, bits, left >= QT, a.d);
+        St::put(to + QT * M::PITCH, rg, bits, left >= QT, a.d);
+        if (threadIdx.x < 2 * QT) reinterpret_cast<float*>(to + 2 * QT * M::PITCH)[threadIdx.x] = -r_stat;
+    };
+    int t = split * per;
+    if (t < end) {
+        fetch_tile(t);
+        put(lds, t);
         __syncthreads();
+    }
+    for (; t < end; ++t) {
+        const char *lds_q = lds + buffer, *lds_g = lds_q + QT * M::PITCH;
+        const float *lds_lse = reinterpret_cast<const float*>(lds_q + 2 * QT * M::PITCH), *lds_delta = lds_lse + QT;
         if (t + 1 < end) fetch_tile(t + 1);
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
@@ -701,7 +741,11 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
             as_operand<T>(y, dp);
             M::mul_t(dk, lds_q, 32 * j, y);
         }
-        __syncthreads();
+        if (t + 1 < end) {
+            put(lds + (OTHER - buffer), t + 1);
+            __syncthreads();
+        }
+        buffer = OTHER - buffer;
     }
     if (key >= a.Nk) return;
     // (a key that is not admitted has gathered the weights that its zeros gave it: nobody else's sum; its gradient is zero)
@@ -788,14 +832,19 @@ Args forward_args(const ogmm_xattn* x, float* ws) {
     return a;
 }
 
+// More than 64 KB of LDS is asked for once a device
+template <class K>
+int allow_lds(K kernel, int bytes, PerDeviceOnce& once) {
+    if (bytes > 65536 && once.first() && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+        return fail("cross attention: %d bytes of LDS are not available", bytes);
+    return 0;
+}
+
 template <class T, int DP, bool KEY_WAVES>
 int launch_fwd(Args a, hipStream_t stream) {
     using S = Fwd<T, DP, KEY_WAVES>;
-    if constexpr (S::LDS > 65536) {
-        static PerDeviceOnce once;
-        if (once.first() && hipFuncSetAttribute(reinterpret_cast<const void*>(&xattn_fwd_kernel<T, DP, KEY_WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess)
-            return fail("ogmm_xattn_fwd: %d bytes of LDS are not available", S::LDS);
-    }
+    static PerDeviceOnce once;
+    if (allow_lds(&xattn_fwd_kernel<T, DP, KEY_WAVES>, S::LDS, once)) return 1;
     const uint32_t grid = deal(a, a.items, static_cast<int64_t>(a.tiles) * a.splits);
     xattn_fwd_kernel<T, DP, KEY_WAVES><<<grid, 256, S::LDS, stream>>>(a);
     if (a.splits > 1) {
@@ -838,7 +887,8 @@ BwdArgs backward_args(const ogmm_xattn* x, float* ws, int64_t* floats) {
 template <class T, int DP>
 int launch_bwd(BwdArgs a, hipStream_t stream) {
     using S = Bwd<T, DP>;
-    static_assert(S::LDS <= 65536, "LDS");
+    static PerDeviceOnce once_q, once_k;
+    if (allow_lds(&xattn_dq_kernel<T, DP>, S::LDS, once_q) || allow_lds(&xattn_dkv_kernel<T, DP>, S::LDS, once_k)) return 1;
     const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
     auto add = [&](const float* part, int parts, int64_t n, void* out) {
         xattn_add_kernel<T><<<static_cast<uint32_t>((n / 4 + 255) / 256), 256, 0, stream>>>(part, parts, n, static_cast<T*>(out));
