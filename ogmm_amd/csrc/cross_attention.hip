@@ -132,10 +132,10 @@ __device__ __forceinline__ uint64_t key_bits(const Args& a, int b, int n0, int l
     return __ballot(n < len && a.key_mask[b * a.mask_b + n]);
 }
 
-// Tiles of KT rows on their way to LDS: 256 threads, sixteen bytes each, CPR chunks to a row.  The rows' addresses are a base that every lane shares and 32 bits of a lane's own.
-template <class T, int DP, int KT>
+// Tiles of KT rows on their way to LDS: sixteen bytes to a thread, CPR chunks to a row.  The rows' addresses are a base that every lane shares and 32 bits of a lane's own.
+template <class T, int DP, int KT, int THREADS>
 struct Stage {
-    static constexpr int CPR = DP * static_cast<int>(sizeof(T)) / 16, STEP = 256 / CPR, PASSES = KT / STEP, PITCH = Tile<T, DP>::PITCH;
+    static constexpr int CPR = DP * static_cast<int>(sizeof(T)) / 16, STEP = THREADS / CPR, PASSES = KT / STEP, PITCH = Tile<T, DP>::PITCH;
     static_assert(PASSES >= 1 && KT % STEP == 0, "shape");
 
     static __device__ __forceinline__ int chunk() { return threadIdx.x % CPR; }
@@ -176,6 +176,17 @@ struct Stage {
         }
     }
 };
+
+// w = 2^(c s - m); -> their sum
+__device__ __forceinline__ float weights(f32x16& w, const f32x16& s, float c, float m) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -m));
+        sum = i ? sum + w[i] : w[i];
+    }
+    return sum;
+}
 
 // A result's start: zeros, or for a lane's sixteen rows 8 (i / 4) + 4 (lane / 32) + i % 4 the values in LDS
 __device__ __forceinline__ f32x16 rows_of(const float* lds) {
@@ -233,23 +244,25 @@ __device__ __forceinline__ void store_one(const ogmm_xattn& a, int64_t at, float
     if (sizeof(T) == 2 && a.rest) static_cast<T*>(a.rest)[at] = static_cast<T>(x - static_cast<float>(v));
 }
 
-template <class T, int DP, bool KEY_WAVES>
+// WAVES of 32 query rows each; KEY_WAVES: one tile of 32 rows, and each of the four waves takes its own 32 keys of a tile
+template <class T, int DP, int WAVES, bool KEY_WAVES>
 struct Fwd {
     // keys of a tile: enough products between two barriers, and so little LDS that two workgroups share a CU
-    static constexpr int KT = KEY_WAVES ? 128 : sizeof(T) == 4 && DP > 64 ? 32 : 64;
+    static constexpr int KT = KEY_WAVES || sizeof(T) * DP * 64 < 1024 * WAVES ? 128 : sizeof(T) == 4 && DP > 64 ? 32 : 64;
     using M = Tile<T, DP>;
-    static constexpr int ROWS = KEY_WAVES ? 32 : 128;
+    static constexpr int ROWS = KEY_WAVES ? 32 : 32 * WAVES, THREADS = 64 * WAVES;
+    static_assert(!KEY_WAVES || WAVES == 4, "shape");
     static constexpr int TILE_BYTES = 2 * KT * M::PITCH + KT * 4;
     // Query waves: two tiles, so that one is written while the other is read, and there is one barrier to a tile; key waves: one, and the four waves' sums side by side at the end
     static constexpr int BUFFERS = KEY_WAVES ? 1 : 2;
     static constexpr int LDS = KEY_WAVES ? std::max(TILE_BYTES, 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8) : BUFFERS * TILE_BYTES;
 };
 
-template <class T, int DP, bool KEY_WAVES>
-__global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) void xattn_fwd_kernel(const Args a) {
-    using S = Fwd<T, DP, KEY_WAVES>;
+template <class T, int DP, int WAVES, bool KEY_WAVES>
+__global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81920 ? 1 : sizeof(T) * DP <= 128 && !KEY_WAVES ? 4 : 2)) void xattn_fwd_kernel(const Args a) {
+    using S = Fwd<T, DP, WAVES, KEY_WAVES>;
     using M = typename S::M;
-    using St = Stage<T, DP, S::KT>;
+    using St = Stage<T, DP, S::KT, S::THREADS>;
     constexpr int KT = S::KT, WORDS = KT > 64 ? KT / 64 : 1, BLOCKS = KEY_WAVES ? 1 : KT / 32, DB = M::DB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // a tile: keys, values, and 0 or -inf for a key that is not admitted
@@ -321,44 +334,35 @@ __global__ __launch_bounds__(256, (Fwd<T, DP, KEY_WAVES>::LDS > 81920 ? 1 : 2)) 
         t = next(t + 1);
         more = t < end;
         if (more) fetch(t);
-        f32x16 s[BLOCKS];
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
             const int key0 = KEY_WAVES ? wave * 32 : 32 * j;
-            s[j] = f32x16{};
-            if (all) mma(s[j], M::row_chunk(lds_k, key0, 0), q[0], T());
-            else mma(s[j] = rows_of(lds_bias + key0), M::row_chunk(lds_k, key0, 0), q[0], T());
+            f32x16 s = {};
+            if (all) mma(s, M::row_chunk(lds_k, key0, 0), q[0], T());
+            else mma(s = rows_of(lds_bias + key0), M::row_chunk(lds_k, key0, 0), q[0], T());
 #pragma unroll
-            for (int u = 1; u < M::CHUNKS; ++u) mma(s[j], M::row_chunk(lds_k, key0, u), q[u], T());
-        }
-        float top = s[0][0];
+            for (int u = 1; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_k, key0, u), q[u], T());
+            // Weights against the maximum that the sums stand at.  Where it is too low, their sum tells: only then is the tile's maximum sought and the sums brought to it.
+            // A weight up to 2^12 keeps its relative precision in every type; what falls below the type's range is 2^-12 of that again.
+            f32x16 w;
+            float part = weights(w, s, c, m);
+            if (__ballot(!(part <= 4096.0f))) {
+                float top = s[0];
 #pragma unroll
-        for (int j = 0; j < BLOCKS; ++j)
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+                const float up = fmaxf(m, max_halves(top) * c), f = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                l *= f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[j][i]);
-        top = max_halves(top) * c;
-        // The sums are brought to a new maximum only where it rose by more than 2^8: weights up to 2^8 keep their relative precision in every type
-        if (__ballot(top > m + 8.0f)) {
-            const float up = fmaxf(m, top), f = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - up);
-            m = up;
-            l *= f;
+                for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[db][i] *= f;
-        }
-        const float shift = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int j = 0; j < BLOCKS; ++j) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], c, -shift));
+                    for (int i = 0; i < 16; ++i) o[db][i] *= f;
+                part = weights(w, s, c, m == -INFINITY ? 0.0f : m);
+            }
+            l += part;          // (of the weights as they are in 32 bits: lse is what the backward's weights are made of)
             u32x4 p[sizeof(T) == 4 ? 4 : 2];
-            as_operand<T>(p, s[j]);
-            float part = 0.0f;          // (of the weights as they are in 32 bits: lse is what the backward's weights are made of)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) part += s[j][i];
-            l += part;
-            M::mul_t(o, lds_v, KEY_WAVES ? wave * 32 : 32 * j, p);
+            as_operand<T>(p, w);
+            M::mul_t(o, lds_v, key0, p);
         }
         if constexpr (S::BUFFERS == 1) __syncthreads();
         if (more) put(lds + (OTHER - buffer));
@@ -533,7 +537,7 @@ template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
     using M = typename S::M;
-    using St = Stage<T, DP, S::KT>;
+    using St = Stage<T, DP, S::KT, 256>;
     constexpr int KT = S::KT, BLOCKS = KT / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     uint32_t buffer = 0;          // where in LDS the tile that is read begins; the other: OTHER - buffer
@@ -639,7 +643,7 @@ template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
     using M = typename S::M;
-    using St = Stage<T, DP, S::KT>;
+    using St = Stage<T, DP, S::KT, 256>;
     constexpr int QT = S::KT, BLOCKS = QT / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // a tile: rows of q, of dout, their -lse, their -delta
@@ -805,8 +809,12 @@ int parts_for(int64_t tiles, int64_t n, int64_t slots) {
     return best;
 }
 
-// Up to 32 query rows of a key head (single tokens): one row tile, and the four waves of its workgroup take different keys.
-bool few_rows(const ogmm_xattn* a) { return static_cast<int64_t>(a->Nq) * (a->H / a->Hkv) <= 32; }
+// Rows of a workgroup's tile.  Up to 32 rows of a key head (single tokens): one tile, whose four waves take different keys.  Eight waves share a tile's keys, which halves what each
+// does to bring them to LDS, where there are rows enough to fill the CUs with them.
+int tile_rows(const ogmm_xattn* a) {
+    const int64_t rows = static_cast<int64_t>(a->Nq) * (a->H / a->Hkv);
+    return rows <= 32 ? 32 : rows * a->Hkv * a->B >= 256 * 256 && rows >= 256 ? 256 : 128;
+}
 
 // -> the grid; per_head: the workgroups of one key head
 uint32_t deal(Args& a, int64_t items, int64_t per_head) {
@@ -821,14 +829,14 @@ Args forward_args(const ogmm_xattn* x, float* ws) {
     static_cast<ogmm_xattn&>(a) = *x;
     a.G = a.H / a.Hkv;
     a.rows = a.Nq * a.G;
-    const int tile_rows = few_rows(x) ? 32 : 128;
-    a.tiles = (a.rows + tile_rows - 1) / tile_rows;
+    const int in_tile = tile_rows(x);
+    a.tiles = (a.rows + in_tile - 1) / in_tile;
     // Where the row tiles alone do not give every CU two workgroups, the keys are cut
     const int64_t base = static_cast<int64_t>(a.B) * a.Hkv * a.tiles;
-    a.splits = parts_for(base, a.Nk, 512);
+    a.splits = parts_for(base, a.Nk, in_tile == 256 ? 256 : 512);
     a.items = static_cast<uint32_t>(base * a.splits);
     a.part_ml = ws;
-    a.part = ws ? ws + static_cast<int64_t>(a.items) * tile_rows * 2 : nullptr;
+    a.part = ws ? ws + static_cast<int64_t>(a.items) * in_tile * 2 : nullptr;
     return a;
 }
 
@@ -840,13 +848,13 @@ int allow_lds(K kernel, int bytes, PerDeviceOnce& once) {
     return 0;
 }
 
-template <class T, int DP, bool KEY_WAVES>
+template <class T, int DP, int WAVES, bool KEY_WAVES>
 int launch_fwd(Args a, hipStream_t stream) {
-    using S = Fwd<T, DP, KEY_WAVES>;
+    using S = Fwd<T, DP, WAVES, KEY_WAVES>;
     static PerDeviceOnce once;
-    if (allow_lds(&xattn_fwd_kernel<T, DP, KEY_WAVES>, S::LDS, once)) return 1;
+    if (allow_lds(&xattn_fwd_kernel<T, DP, WAVES, KEY_WAVES>, S::LDS, once)) return 1;
     const uint32_t grid = deal(a, a.items, static_cast<int64_t>(a.tiles) * a.splits);
-    xattn_fwd_kernel<T, DP, KEY_WAVES><<<grid, 256, S::LDS, stream>>>(a);
+    xattn_fwd_kernel<T, DP, WAVES, KEY_WAVES><<<grid, S::THREADS, S::LDS, stream>>>(a);
     if (a.splits > 1) {
         const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.rows;
         xattn_join_kernel<T><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, stream>>>(a, S::ROWS);
@@ -946,7 +954,7 @@ extern "C" int64_t ogmm_xattn_workspace_bytes(const ogmm_xattn* a, int backward)
         return floats * static_cast<int64_t>(sizeof(float));
     }
     const Args f = forward_args(a, nullptr);
-    return f.splits > 1 ? static_cast<int64_t>(f.items) * (few_rows(a) ? 32 : 128) * (a->d + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+    return f.splits > 1 ? static_cast<int64_t>(f.items) * tile_rows(a) * (a->d + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
 extern "C" int ogmm_xattn_fwd(const ogmm_xattn* x, void* stream) {
@@ -954,12 +962,12 @@ extern "C" int ogmm_xattn_fwd(const ogmm_xattn* x, void* stream) {
     if (!x->B || !x->Nq) return 0;
     const Args a = forward_args(x, static_cast<float*>(x->workspace));
     OGMM_REQUIRE(a.splits == 1 || a.workspace, "ogmm_xattn_fwd: missing workspace");
-    const bool few = few_rows(x);
+    const int rows = tile_rows(x);
     return with_type(x->type, [&](auto t) {
         return with_width(x->d, [&](auto w) {
             using T = decltype(t);
             constexpr int DP = decltype(w)::value;
-            return few ? launch_fwd<T, DP, true>(a, as_stream(stream)) : launch_fwd<T, DP, false>(a, as_stream(stream));
+            return rows == 32 ? launch_fwd<T, DP, 4, true>(a, as_stream(stream)) : rows == 128 ? launch_fwd<T, DP, 4, false>(a, as_stream(stream)) : launch_fwd<T, DP, 8, false>(a, as_stream(stream));
         });
     });
 }
