@@ -125,11 +125,14 @@ __device__ __forceinline__ float add_halves(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Which of the 64 keys from n0 are admitted, one bit each (the same in every wave)
-__device__ __forceinline__ uint64_t key_bits(const Args& a, int b, int n0, int len) {
-    if (!a.key_mask) return len - n0 >= 64 ? ~uint64_t(0) : len > n0 ? (uint64_t(1) << (len - n0)) - 1 : 0;
+// Which keys are admitted, 64 at a time, one bit each: a lane's byte of the mask is on its way with the tile's keys, the bits are taken when both have come
+__device__ __forceinline__ uint8_t mask_byte(const Args& a, int b, int n0, int len) {
     const int n = n0 + (threadIdx.x & 63);
-    return __ballot(n < len && a.key_mask[b * a.mask_b + n]);
+    return a.key_mask && n < len ? a.key_mask[b * a.mask_b + n] : 0;
+}
+__device__ __forceinline__ uint64_t key_bits(const Args& a, uint8_t byte, int n0, int len) {
+    if (a.key_mask) return __ballot(byte);
+    return len - n0 >= 64 ? ~uint64_t(0) : len > n0 ? (uint64_t(1) << (len - n0)) - 1 : 0;
 }
 
 // Tiles of KT rows on their way to LDS: sixteen bytes to a thread, CPR chunks to a row.  The rows' addresses are a base that every lane shares and 32 bits of a lane's own.
@@ -231,11 +234,20 @@ __device__ __forceinline__ void store_column(T* __restrict__ out, T* __restrict_
 }
 template <class M>
 __device__ __forceinline__ void store_part(float* __restrict__ out, const f32x16 (&c)[M::DB], float f, int d) {
+    if constexpr (M::ROW == 2 * 32 * M::DB) {
 #pragma unroll
-    for (int db = 0; db < M::DB; ++db)
+        for (int db = 0; db < M::DB; ++db)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (M::channel(db, i) < d) out[M::channel(db, i)] = c[db][i] * f;
+            for (int i = 0; i < 16; i += 4)
+                if (M::channel(db, i) < d) *reinterpret_cast<float4*>(out + M::channel(db, i)) = make_float4(c[db][i] * f, c[db][i + 1] * f, c[db][i + 2] * f, c[db][i + 3] * f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (M::channel(0, i) >= d) continue;
+#pragma unroll
+            for (int db = 0; db < M::DB; ++db) out[M::channel(db, i)] = c[db][i] * f;
+        }
+    }
 }
 template <class T>
 __device__ __forceinline__ void store_one(const ogmm_xattn& a, int64_t at, float x) {
@@ -296,44 +308,42 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
     float m = -INFINITY, l = 0.0f;          // m: of scale S log2(e), the running maximum or up to 8 below it
     f32x16 o[DB] = {};
     u32x4 rk[St::PASSES], rv[St::PASSES];
-    uint64_t next_bits[WORDS];
-    auto next = [&](int t) {          // the first tile from t on that has an admitted key
-        for (; t < end; ++t) {
-            uint64_t any = 0;
-#pragma unroll
-            for (int w = 0; w < WORDS; ++w) any |= next_bits[w] = key_bits(a, b, t * KT + 64 * w, KT < 64 ? min(len, (t + 1) * KT) : len);
-            if (any) break;
-        }
-        return t;
-    };
+    uint8_t bytes[WORDS];
     auto fetch = [&](int t) {
         St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
         St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
-    };
-    bool full = true;
-    auto put = [&](char* to) {          // (what next() found out about the tile goes with it)
-        full = true;
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w) full &= next_bits[w] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
-        St::put(to, rk, next_bits, full, a.d);
-        St::put(to + KT * M::PITCH, rv, next_bits, full, a.d);
-        if (!full && threadIdx.x < KT)
-            reinterpret_cast<float*>(to + 2 * KT * M::PITCH)[threadIdx.x] = next_bits[WORDS == 1 ? 0 : threadIdx.x >> 6] >> (threadIdx.x & 63) & 1 ? 0.0f : -INFINITY;
+        for (int w = 0; w < WORDS; ++w) bytes[w] = mask_byte(a, b, t * KT + 64 * w, min(len, (t + 1) * KT));
     };
-    int t = next(split * per);
-    bool more = t < end;
-    if (more) {
+    bool full = true, any = true;
+    auto put = [&](char* to, int t) {
+        uint64_t bits[WORDS], all = ~uint64_t(0), one = 0;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+            bits[w] = key_bits(a, bytes[w], t * KT + 64 * w, min(len, (t + 1) * KT));
+            all &= bits[w];
+            one |= bits[w];
+        }
+        full = all == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
+        any = one != 0;
+        St::put(to, rk, bits, full, a.d);
+        St::put(to + KT * M::PITCH, rv, bits, full, a.d);
+        if (!full && threadIdx.x < KT)
+            reinterpret_cast<float*>(to + 2 * KT * M::PITCH)[threadIdx.x] = bits[WORDS == 1 ? 0 : threadIdx.x >> 6] >> (threadIdx.x & 63) & 1 ? 0.0f : -INFINITY;
+    };
+    int t = split * per;
+    if (t < end) {
         fetch(t);
-        put(lds);
+        put(lds, t);
         __syncthreads();
     }
-    while (more) {
-        const bool all = full;
+    for (; t < end; ++t) {
+        // (flags are the same in every lane, and known to be: matrix instructions take no notice of lanes that a branch left out)
+        const bool all = __builtin_amdgcn_readfirstlane(full), some = __builtin_amdgcn_readfirstlane(any);
         const char *lds_k = lds + buffer, *lds_v = lds_k + KT * M::PITCH;
         const float* lds_bias = reinterpret_cast<const float*>(lds_k + 2 * KT * M::PITCH);
-        t = next(t + 1);
-        more = t < end;
-        if (more) fetch(t);
+        if (t + 1 < end) fetch(t + 1);
+        if (some)
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
             const int key0 = KEY_WAVES ? wave * 32 : 32 * j;
@@ -365,8 +375,8 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
             M::mul_t(o, lds_v, key0, p);
         }
         if constexpr (S::BUFFERS == 1) __syncthreads();
-        if (more) put(lds + (OTHER - buffer));
-        if (more || KEY_WAVES) __syncthreads();
+        if (t + 1 < end) put(lds + (OTHER - buffer), t + 1);
+        if (t + 1 < end || KEY_WAVES) __syncthreads();
         buffer = OTHER - buffer;
     }
     l = add_halves(l);
@@ -534,7 +544,7 @@ struct Bwd {
 };
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 128 ? 2 : 3)) void xattn_dq_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
     using M = typename S::M;
     using St = Stage<T, DP, S::KT, 256>;
@@ -576,40 +586,36 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
     const int tiles = tile * 128 < q_rows ? (len + KT - 1) / KT : 0, per = (tiles + a.row_splits - 1) / a.row_splits, end = min(tiles, (split + 1) * per);
     f32x16 dq[M::DB] = {};
     u32x4 rk[St::PASSES], rv[St::PASSES];
-    uint64_t next_bits[1] = {0};
-    auto next = [&](int t) {
-        for (; t < end; ++t)
-            if ((next_bits[0] = key_bits(a, b, t * KT, min(len, (t + 1) * KT)))) break;
-        return t;
-    };
+    uint8_t byte;
     auto fetch = [&](int t) {
         St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
         St::fetch(rv, v, v_step, t * KT, a.Nk, chunk_off);
+        byte = mask_byte(a, b, t * KT, min(len, (t + 1) * KT));
     };
-    bool full = true;
-    auto put = [&](char* to) {
-        full = next_bits[0] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
-        St::put(to, rk, next_bits, full, a.d);
-        St::put(to + KT * M::PITCH, rv, next_bits, full, a.d);
-        if (!full && threadIdx.x < KT) reinterpret_cast<float*>(to + 2 * KT * M::PITCH)[threadIdx.x] = next_bits[0] >> threadIdx.x & 1 ? 0.0f : -INFINITY;
+    bool full = true, any = true;
+    auto put = [&](char* to, int t) {
+        const uint64_t bits[1] = {key_bits(a, byte, t * KT, min(len, (t + 1) * KT))};
+        full = bits[0] == (KT < 64 ? (uint64_t(1) << (KT & 63)) - 1 : ~uint64_t(0));
+        any = bits[0] != 0;
+        St::put(to, rk, bits, full, a.d);
+        St::put(to + KT * M::PITCH, rv, bits, full, a.d);
+        if (!full && threadIdx.x < KT) reinterpret_cast<float*>(to + 2 * KT * M::PITCH)[threadIdx.x] = bits[0] >> threadIdx.x & 1 ? 0.0f : -INFINITY;
     };
     f32x16 start;          // dP - delta from the start
 #pragma unroll
     for (int i = 0; i < 16; ++i) start[i] = -delta;
-    int t = next(split * per);
-    bool more = t < end;
-    if (more) {
+    int t = split * per;
+    if (t < end) {
         fetch(t);
-        put(lds);
+        put(lds, t);
         __syncthreads();
     }
-    while (more) {
-        const bool all = full;
+    for (; t < end; ++t) {
+        const bool all = __builtin_amdgcn_readfirstlane(full), some = __builtin_amdgcn_readfirstlane(any);          // (see the forward)
         const char *lds_k = lds + buffer, *lds_v = lds_k + KT * M::PITCH;
         const float* lds_bias = reinterpret_cast<const float*>(lds_k + 2 * KT * M::PITCH);
-        t = next(t + 1);
-        more = t < end;
-        if (more) fetch(t);
+        if (t + 1 < end) fetch(t + 1);
+        if (some)
 #pragma unroll
         for (int j = 0; j < BLOCKS; ++j) {
             f32x16 s = {}, dp = start;
@@ -625,8 +631,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void xattn_dq_
             as_operand<T>(ds, s);
             M::mul_t(dq, lds_k, 32 * j, ds);
         }
-        if (more) {
-            put(lds + (OTHER - buffer));
+        if (t + 1 < end) {
+            put(lds + (OTHER - buffer), t + 1);
             __syncthreads();
         }
         buffer = OTHER - buffer;
@@ -657,7 +663,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
     const int key = tile * 128 + wave * 32 + (lane & 31);
     const bool key_there = key < len && (!a.key_mask || a.key_mask[b * a.mask_b + key]);
     // (all four waves take part in the tiles of rows, or none: a tile of keys without one that is admitted)
-    const bool any = (key_bits(a, b, tile * 128, len) | key_bits(a, b, tile * 128 + 64, len)) != 0;
+    const bool any = (key_bits(a, mask_byte(a, b, tile * 128, len), tile * 128, len) | key_bits(a, mask_byte(a, b, tile * 128 + 64, len), tile * 128 + 64, len)) != 0;
     const float c = a.scale * LOG2E, up = gradient_scale<T>(a, bh);
     u32x4 k[M::CHUNKS], v[M::CHUNKS];
     {
@@ -813,7 +819,8 @@ int parts_for(int64_t tiles, int64_t n, int64_t slots) {
 // does to bring them to LDS, where there are rows enough to fill the CUs with them.
 int tile_rows(const ogmm_xattn* a) {
     const int64_t rows = static_cast<int64_t>(a->Nq) * (a->H / a->Hkv);
-    return rows <= 32 ? 32 : rows * a->Hkv * a->B >= 256 * 256 && rows >= 256 ? 256 : 128;
+    const bool narrow = a->d * (a->type == OGMM_F32 ? 2 : 1) <= 64;
+    return rows <= 32 ? 32 : narrow && rows * a->Hkv * a->B >= 256 * 256 && rows >= 256 ? 256 : 128;
 }
 
 // -> the grid; per_head: the workgroups of one key head
