@@ -52,11 +52,11 @@ __device__ __forceinline__ void mma(f32x16& c, u32x4 a, u32x4 b, float) {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
 }
 
-// A matrix of rows in LDS.  The gap sets neighbouring rows sixteen bytes apart in the banks: of 0, 16, 32, 48, 64 bytes it costs the row reads least (181, against 202 cycles for four
-// dependent ones without it, 301 at rows of 256 bytes), and the transposing reads do not mind.
+// A matrix of rows in LDS, with a gap between rows that keeps both of its readers off each other's banks.  Clocks of a CU for a wave's instruction, eight waves, at gaps of 0, 16, 32
+// and 48 bytes: sixteen bytes of each of 32 rows 64.1, 4.7, 8.1, 4.6 (rows of 256 bytes) and 16.1, 5.6, 5.3, 5.4 (128 bytes); transposing reads 8.1, 8.2, 4.3, 4.2 and 4.3, 4.2, 4.3, 4.5.
 template <class T, int DP>
 struct Tile {
-    static constexpr int ROW = DP * sizeof(T), PITCH = ROW + 16, CHUNKS = ROW / 32, DB = DP / 32;
+    static constexpr int ROW = DP * sizeof(T), PITCH = ROW + (ROW == 256 ? 48 : 16), CHUNKS = ROW / 32, DB = DP / 32;
 
     // row lane % 32 of a block of 32 rows, chunk s of its channels
     static __device__ __forceinline__ u32x4 row_chunk(const char* lds, int row0, int s) {
