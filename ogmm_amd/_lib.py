@@ -153,9 +153,9 @@ PROTOTYPES = {
     "ogmm_scatter_add_rows": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p],
     "ogmm_small_bmm_nt": [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p],
     "ogmm_l2norm_rows_bwd": [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p],
-    "ogmm_xattn_workspace_bytes": [POINTER(XattnDesc), c_int],
-    "ogmm_xattn_fwd": [POINTER(XattnDesc), c_void_p],
-    "ogmm_xattn_bwd": [POINTER(XattnDesc), c_void_p],
+    "ogmm_xattn_workspace_bytes": [c_void_p, c_int],          # struct ogmm_xattn*
+    "ogmm_xattn_fwd": [c_void_p, c_void_p],
+    "ogmm_xattn_bwd": [c_void_p, c_void_p],
     "ogmm_rms_norm": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
     "ogmm_rms_norm_q8": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "ogmm_rms_norm_bwd_workspace_bytes": [c_int64, c_int],

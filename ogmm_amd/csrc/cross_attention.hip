@@ -802,12 +802,12 @@ int with_width(int d, F&& f) {
     return f(integral_constant<int, 128>());
 }
 
-// Into how many parts the other sequence's n rows are cut, for `tiles` workgroups on a part that holds `slots` of them at once: parts of 256 rows at least, as many as shorten
+// Into how many parts the other sequence's n rows are cut, for `tiles` workgroups on a part that holds `slots` of them at once: parts of least_rows at least, as many as shorten
 // the sum of the rounds by more than a part costs in writing and joining (taken as 1/16 of a round of it).
-int parts_for(int64_t tiles, int64_t n, int64_t slots) {
+int parts_for(int64_t tiles, int64_t n, int64_t slots, int64_t least_rows = 256) {
     int best = 1;
     double least = 1e30;
-    for (int64_t s = 1; s <= std::min<int64_t>((n + 255) / 256, 512); ++s) {
+    for (int64_t s = 1; s <= std::min<int64_t>((n + least_rows - 1) / least_rows, 512); ++s) {
         const double t = static_cast<double>((tiles * s + slots - 1) / slots) / s + (s > 1 ? s * tiles / (16.0 * slots) : 0.0);
         if (t < least * 0.999) { least = t; best = static_cast<int>(s); }
         if (tiles * s > 4 * slots) break;
@@ -840,7 +840,7 @@ Args forward_args(const ogmm_xattn* x, float* ws) {
     a.tiles = (a.rows + in_tile - 1) / in_tile;
     // Where the row tiles alone do not give every CU two workgroups, the keys are cut
     const int64_t base = static_cast<int64_t>(a.B) * a.Hkv * a.tiles;
-    a.splits = parts_for(base, a.Nk, in_tile == 256 ? 256 : 512);
+    a.splits = parts_for(base, a.Nk, in_tile == 256 ? 256 : 512, in_tile == 32 ? 128 : 256);          // (128 keys: one tile of the key waves)
     a.items = static_cast<uint32_t>(base * a.splits);
     a.part_ml = ws;
     a.part = ws ? ws + static_cast<int64_t>(a.items) * in_tile * 2 : nullptr;

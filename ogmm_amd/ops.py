@@ -2,7 +2,9 @@
 device memory and the stream; every function enqueues HIP kernels of libogmm_hip.so on torch's current
 stream and returns without synchronising.  All tensors must be CUDA (ROCm) tensors -- there is no CPU path.
 """
+import array
 import ctypes
+import struct
 
 import torch
 
@@ -1172,14 +1174,15 @@ def weight_grad_thin(dy, x, split=False, overflow=None):
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # OGMM_F32 / OGMM_BF16 / OGMM_F16
 
 
-def _dev(name, first, *others):
-    """The device of a call's tensors: all on one GPU, of a type that has kernels; others: (name, tensor or None)."""
+def _dev(name, first, **others):
+    """The device of a call's tensors, all on one GPU; others: by name, tensors or None"""
     if not isinstance(first, torch.Tensor) or not first.is_cuda:
         raise _lib.OgmmError("%s must be a CUDA/ROCm tensor (the HIP path has no CPU fallback)" % name)
-    for n, t in others:
-        if t is not None and (not isinstance(t, torch.Tensor) or t.device != first.device):
-            raise _lib.OgmmError("%s must be a tensor on %s" % (n, first.device))
-    return first.device
+    dev = first.device
+    for n, t in others.items():
+        if t is not None and (not isinstance(t, torch.Tensor) or t.device != dev):
+            raise _lib.OgmmError("%s must be a tensor on %s" % (n, dev))
+    return dev
 
 
 def _code(t, name):
@@ -1191,71 +1194,79 @@ def _code(t, name):
 
 def _call_on(dev, name, *args):
     """_lib.call on the tensors' own device and on torch's current stream OF that device, whichever device is current (the stream comes last)."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
-        return
-    with torch.cuda.device(dev):
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise _lib.OgmmError("%s failed: %s" % (name, _lib.load().ogmm_last_error().decode(errors="replace")))
 
 
-def _heads(t, name, like=None):
-    """[B, n, heads, d] as the attention kernels take it: channels contiguous, address and strides multiples of 16 bytes (anything else is copied)"""
-    if t.dim() != 4:
-        raise _lib.OgmmError("%s must be [B, n, heads, d], got %s" % (name, tuple(t.shape)))
-    if like is not None and t.dtype != like.dtype:
-        raise _lib.OgmmError("%s must be %s, got %s" % (name, like.dtype, t.dtype))
+def _heads(t, name, dtype):
+    """[B, n, heads, d] as the attention kernels take it -> (tensor, its strides of batch, row and head): channels contiguous, address and strides multiples of
+    16 bytes, rows and heads less than 32 MB apart; anything else is copied"""
+    if t.dim() != 4 or t.dtype != dtype:
+        raise _lib.OgmmError("%s must be %s [B, n, heads, d], got %s %s" % (name, dtype, t.dtype, tuple(t.shape)))
+    B, N, H, D = t.shape
     b, n, h, one = t.stride()
-    step = 16 // t.element_size()
-    if (one != 1 and t.shape[3] != 1) or (b | n | h) % step or t.data_ptr() % 16 or max(n, h) * t.element_size() >= 1 << 25:
-        t = t.contiguous()
-        if t.data_ptr() % 16:          # (contiguous already, at an odd address)
-            t = t.clone()
-    return t
+    b, n, h = b if B > 1 else 0, n if N > 1 else 0, h if H > 1 else 0
+    e = t.element_size()
+    if (one != 1 and D > 1) or (b | n | h) * e % 16 or t.data_ptr() % 16 or n * e >= 1 << 25 or h * e >= 1 << 25:
+        t = torch.empty((B, N, H, D), dtype=dtype, device=t.device).copy_(t)
+        b, n, h = N * H * D, H * D, D
+    return t, b, n, h
 
 
 def _lens(t, B, name):
     if t is None:
         return None
-    if _i32(t, name).shape != (B,):
-        raise _lib.OgmmError("%s must have one entry for each of the %d batch entries, got %s" % (name, B, tuple(t.shape)))
+    if t.dtype != torch.int32 or t.shape != (B,):
+        raise _lib.OgmmError("%s must be int32 with one entry for each of the %d batch entries, got %s %s" % (name, B, t.dtype, tuple(t.shape)))
     return t.contiguous()
 
 
-def _xattn(q, k, v, kv_lens, q_lens, key_mask, scale):
-    dev = _dev("q", q, ("k", k), ("v", v), ("kv_lens", kv_lens), ("q_lens", q_lens), ("key_mask", key_mask))
-    code = _code(q, "q")
-    q, k, v = _heads(q, "q"), _heads(k, "k", q), _heads(v, "v", q)
-    B, Nq, H, d = q.shape
-    Nk, Hkv = k.shape[1:3]
-    if k.shape != (B, Nk, Hkv, d) or v.shape != k.shape:
-        raise _lib.OgmmError("q %s, k %s and v %s do not fit: [B, Nq, H, d] and twice [B, Nk, Hkv, d]" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    kv_lens, q_lens = _lens(kv_lens, B, "kv_lens"), _lens(q_lens, B, "q_lens")
-    if key_mask is not None:
-        if key_mask.shape != (B, Nk) or key_mask.dtype != torch.bool:
-            raise _lib.OgmmError("key_mask must be bool [%d, %d], got %s %s" % (B, Nk, key_mask.dtype, tuple(key_mask.shape)))
-        if key_mask.stride(1) != 1:
-            key_mask = key_mask.contiguous()
-    a = _lib.XattnDesc()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_b, a.q_n, a.q_h, _ = q.stride()
-    a.k_b, a.k_n, a.k_h, _ = k.stride()
-    a.v_b, a.v_n, a.v_h, _ = v.stride()
-    a.B, a.Nq, a.Nk, a.H, a.Hkv, a.d, a.type = B, Nq, Nk, H, Hkv, d, code
-    a.scale = d ** -0.5 if scale is None else scale
-    a.q_lens = None if q_lens is None else q_lens.data_ptr()
-    a.kv_lens = None if kv_lens is None else kv_lens.data_ptr()
-    if key_mask is not None:
-        a.key_mask, a.mask_b = key_mask.data_ptr(), key_mask.stride(0)
-    return a, dev, (q, k, v, kv_lens, q_lens, key_mask)          # (the tensors: alive until the kernels are enqueued)
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
-def _xattn_call(name, a, dev, backward):
-    nbytes = _lib.load().ogmm_xattn_workspace_bytes(ctypes.byref(a), backward)
-    ws = None
-    if nbytes > 0:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a.workspace = ws.data_ptr()
-    _call_on(dev, name, ctypes.byref(a))
+_XATTN = struct.Struct("3P9q3P7if3PqP3q3PP")          # struct ogmm_xattn (_lib.XattnDesc names its fields): packed in one go, a third of the time of setting them one by one
+
+
+class _Xattn:
+    """The checked arguments of an attention call"""
+    __slots__ = ("dev", "q", "k", "v", "held", "dims", "scale", "mask")
+
+    def __init__(self, q, k, v, kv_lens, q_lens, key_mask, scale):
+        self.dev = _dev("q", q, k=k, v=v, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask)
+        code = _code(q, "q")
+        self.q, self.k, self.v = _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
+        B, Nq, H, d = q.shape
+        Nk, Hkv = k.shape[1:3]
+        if k.shape != (B, Nk, Hkv, d) or v.shape != k.shape:
+            raise _lib.OgmmError("q %s, k %s and v %s do not fit: [B, Nq, H, d] and twice [B, Nk, Hkv, d]" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+        kv_lens, q_lens = _lens(kv_lens, B, "kv_lens"), _lens(q_lens, B, "q_lens")
+        if key_mask is not None:
+            if key_mask.shape != (B, Nk) or key_mask.dtype != torch.bool:
+                raise _lib.OgmmError("key_mask must be bool [%d, %d], got %s %s" % (B, Nk, key_mask.dtype, tuple(key_mask.shape)))
+            if key_mask.stride(1) != 1:
+                key_mask = key_mask.contiguous()
+        self.held = kv_lens, q_lens, key_mask          # (alive until the kernels are enqueued)
+        self.dims = B, Nq, Nk, H, Hkv, d, code
+        self.scale = d ** -0.5 if scale is None else float(scale)
+
+    def call(self, name, backward, o, rest, lse, dout=(None, 0, 0, 0), grads=(None, None, None)):
+        (q, *qs), (k, *ks), (v, *vs), (g, *gs) = self.q, self.k, self.v, dout
+        kv_lens, q_lens, key_mask = self.held
+        head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs, _ptr(o), _ptr(rest), _ptr(lse), *self.dims, self.scale, _ptr(q_lens), _ptr(kv_lens), _ptr(key_mask),
+                0 if key_mask is None else key_mask.stride(0), _ptr(g), *gs, *map(_ptr, grads))
+        desc = _XATTN.pack(*head, 0)
+        nbytes = _lib.load().ogmm_xattn_workspace_bytes(desc, backward)
+        if nbytes > 0:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.dev)
+            desc = _XATTN.pack(*head, ws.data_ptr())
+        _call_on(self.dev, name, desc)
 
 
 def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=None, need_lse=False, need_rest=False):
@@ -1266,54 +1277,55 @@ def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=Non
     what stands in keys that are not admitted does not matter.  -> o [B, Nq, H, d], with need_lse also log sum exp of the scores, fp32 [B, H, Nq] (-inf for such rows).
     need_rest (for the backward, with need_lse): -> (o, lse, rest), rest = what rounding to 16 bits left of o, in the type again (None for float32).
     One row or a few against many keys are split over the keys.  For attention to at most 128 anchors of equal clouds see attention()."""
-    a, dev, held = _xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
-    o = torch.empty(held[0].shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((a.B, a.H, a.Nq), dtype=torch.float32, device=dev) if need_lse else None
-    rest = torch.empty_like(o) if need_rest and a.type else None
-    a.o, a.rest, a.lse = o.data_ptr(), None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr()
-    _xattn_call("ogmm_xattn_fwd", a, dev, 0)
+    a = _Xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
+    B, Nq, _, H, *_, code = a.dims
+    o = q.new_empty(q.shape)
+    lse = q.new_empty((B, H, Nq), dtype=torch.float32) if need_lse else None
+    rest = torch.empty_like(o) if need_rest and code else None
+    a.call("ogmm_xattn_fwd", 0, o, rest, lse)
     return (o, lse, rest) if need_rest else (o, lse) if need_lse else o
 
 
 def cross_attention_bwd(q, k, v, o, lse, dout, kv_lens=None, q_lens=None, key_mask=None, scale=None, rest=None):
     """Backward of cross_attention(): (dq, dk, dv) from dout = dL/do and the forward's o and lse (and rest); the scores are formed again.  Gradients of a key head are summed over
     the query heads that share it; keys that are not admitted and rows behind q_lens get zeros.  Repeated calls agree bit for bit."""
-    a, dev, held = _xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
-    _dev("q", held[0], ("o", o), ("lse", lse), ("dout", dout), ("rest", rest))
-    if o.shape != held[0].shape or dout.shape != held[0].shape or lse.shape != (a.B, a.H, a.Nq):
+    a = _Xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
+    _dev("q", q, o=o, lse=lse, dout=dout, rest=rest)
+    B, Nq, _, H, *_, code = a.dims
+    if o.shape != q.shape or dout.shape != q.shape or lse.shape != (B, H, Nq):
         raise _lib.OgmmError("o %s, dout %s and lse %s must be shaped as cross_attention() returns them for q %s" % (tuple(o.shape), tuple(dout.shape), tuple(lse.shape), tuple(q.shape)))
     if o.dtype != q.dtype or rest is not None and (rest.dtype != q.dtype or rest.shape != o.shape):
         raise _lib.OgmmError("o and rest must be %s %s, got %s and %s" % (q.dtype, tuple(o.shape), o.dtype, None if rest is None else (rest.dtype, tuple(rest.shape))))
-    if rest is not None and a.type:
-        rest = _heads(rest.contiguous(), "rest")
-        a.rest = rest.data_ptr()
-    dout, o, lse = _heads(dout, "dout", q), _heads(o.contiguous(), "o"), _f32(lse, "lse").contiguous()
-    dq = torch.empty(held[0].shape, dtype=q.dtype, device=dev)
-    dk, dv = (torch.empty(held[1].shape, dtype=q.dtype, device=dev) for _ in range(2))
-    a.o, a.lse, a.dout = o.data_ptr(), lse.data_ptr(), dout.data_ptr()
-    a.do_b, a.do_n, a.do_h, _ = dout.stride()
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    _xattn_call("ogmm_xattn_bwd", a, dev, 1)
+    o, rest = (None if t is None else _heads(t.contiguous(), "o", q.dtype)[0] for t in (o, rest if code else None))
+    lse = _f32(lse, "lse").contiguous()
+    dq = q.new_empty(q.shape)
+    dk = k.new_empty(k.shape)
+    dv = k.new_empty(k.shape)
+    a.call("ogmm_xattn_bwd", 1, o, rest, lse, _heads(dout, "dout", q.dtype), (dq, dk, dv))
     return dq, dk, dv
 
 
-def _rows(t, D, name):
+def _rows(t, D):
     """[..., D] as rows with contiguous values -> (2-D view or copy, row stride)"""
-    t = t.reshape(-1, D)
-    if t.stride(1) != 1 and D != 1:
+    if t.dim() != 2:
+        t = t.reshape(-1, D)
+    step, one = t.stride()
+    if one != 1 and D != 1:
         t = t.contiguous()
-    return t, t.stride(0)
+        step = D
+    return t, step
 
 
 def _norm_args(x, weight, residual):
-    dev = _dev("x", x, ("weight", weight), ("residual", residual))
+    dev = _dev("x", x, weight=weight, residual=residual)
     code = _code(x, "x")
-    if x.dim() < 1 or not x.shape[-1] or weight.shape != x.shape[-1:]:
-        raise _lib.OgmmError("weight must have one value for each of the last axis of x %s, got %s" % (tuple(x.shape), tuple(weight.shape)))
+    shape = x.shape
+    if not shape or not shape[-1] or weight.shape != shape[-1:]:
+        raise _lib.OgmmError("weight must have one value for each of the last axis of x %s, got %s" % (tuple(shape), tuple(weight.shape)))
     if weight.dtype != x.dtype and weight.dtype != torch.float32:
         raise _lib.OgmmError("weight must be %s or float32, got %s" % (x.dtype, weight.dtype))
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise _lib.OgmmError("residual must be %s %s, got %s %s" % (x.dtype, tuple(x.shape), residual.dtype, tuple(residual.shape)))
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
+        raise _lib.OgmmError("residual must be %s %s, got %s %s" % (x.dtype, tuple(shape), residual.dtype, tuple(residual.shape)))
     return dev, code, weight.contiguous()
 
 
@@ -1323,12 +1335,12 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     that rounding); rstd fp32, one value a row, is what rms_norm_bwd() takes."""
     dev, code, w = _norm_args(x, weight, residual)
     D = x.shape[-1]
-    x2, ldx = _rows(x, D, "x")
-    r2, ldr = _rows(residual, D, "residual") if residual is not None else (None, 0)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    _call_on(dev, "ogmm_rms_norm", x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps,
+    x2, ldx = _rows(x, D)
+    r2, ldr = _rows(residual, D) if residual is not None else (None, 0)
+    y = x.new_empty(x.shape)
+    h = x if residual is None else x.new_empty(x.shape)
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _call_on(dev, "ogmm_rms_norm", x2.data_ptr(), ldx, _ptr(r2), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps,
              y.data_ptr(), None if residual is None else h.data_ptr(), rstd.data_ptr())
     return y, h, rstd
 
@@ -1340,12 +1352,12 @@ def rms_norm_q8(x, weight, residual=None, eps=1e-6, group=0):
     if group not in (0, 32, 64, 128):
         raise _lib.OgmmError("group must be 0 (one scale a row), 32, 64 or 128 columns, got %r" % (group,))
     D = x.shape[-1]
-    x2, ldx = _rows(x, D, "x")
-    r2, ldr = _rows(residual, D, "residual") if residual is not None else (None, 0)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    x2, ldx = _rows(x, D)
+    r2, ldr = _rows(residual, D) if residual is not None else (None, 0)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
     scales = torch.empty(x.shape[:-1] + (-(-D // group) if group else 1,), dtype=torch.float32, device=dev)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    _call_on(dev, "ogmm_rms_norm_q8", x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps, group,
+    h = x if residual is None else x.new_empty(x.shape)
+    _call_on(dev, "ogmm_rms_norm_q8", x2.data_ptr(), ldx, _ptr(r2), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps, group,
              q.data_ptr(), scales.data_ptr(), None if residual is None else h.data_ptr())
     return q, scales, h
 
@@ -1353,17 +1365,17 @@ def rms_norm_q8(x, weight, residual=None, eps=1e-6, group=0):
 def rms_norm_bwd(dy, h, weight, rstd, dh=None):
     """Backward of rms_norm(): (dx, dweight) from dy = dL/dy, the forward's h and rstd, and dh = dL/dh where the sum has readers of its own; dx is the residual's gradient too."""
     dev, code, w = _norm_args(h, weight, None)
-    _dev("h", h, ("dy", dy), ("rstd", rstd), ("dh", dh))
+    _dev("h", h, dy=dy, rstd=rstd, dh=dh)
     for n, t in (("dy", dy), ("dh", dh)):
         if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
             raise _lib.OgmmError("%s must be %s %s, got %s %s" % (n, h.dtype, tuple(h.shape), t.dtype, tuple(t.shape)))
     if _f32(rstd, "rstd").shape != h.shape[:-1]:
         raise _lib.OgmmError("rstd must have one value for each row of h %s, got %s" % (tuple(h.shape), tuple(rstd.shape)))
     D = h.shape[-1]
-    (dy2, lddy), (h2, ldh), rstd = _rows(dy, D, "dy"), _rows(h, D, "h"), rstd.contiguous()
-    dh2, lddh = _rows(dh, D, "dh") if dh is not None else (None, 0)
-    dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
-    dw = torch.empty(D, dtype=w.dtype, device=dev)
+    (dy2, lddy), (h2, ldh), rstd = _rows(dy, D), _rows(h, D), rstd.contiguous()
+    dh2, lddh = _rows(dh, D) if dh is not None else (None, 0)
+    dx = h.new_empty(h.shape)
+    dw = w.new_empty(D)
     ws = torch.empty(_lib.load().ogmm_rms_norm_bwd_workspace_bytes(h2.shape[0], D), dtype=torch.uint8, device=dev)
     _call_on(dev, "ogmm_rms_norm_bwd", dy2.data_ptr(), lddy, h2.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), None if dh2 is None else dh2.data_ptr(), lddh, h2.shape[0], D,
              code, _TYPE[w.dtype], dx.data_ptr(), dw.data_ptr(), ws.data_ptr())
@@ -1372,8 +1384,6 @@ def rms_norm_bwd(dy, h, weight, rstd, dh=None):
 
 def _dense(t):
     """True where a tensor's elements fill one stretch of memory without gaps or overlaps, in any order of its axes"""
-    if t.is_contiguous():
-        return True
     n = 1
     for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s != 1), key=lambda p: p[1]):
         if stride != n:
@@ -1383,20 +1393,20 @@ def _dense(t):
 
 
 def _grad_list(grads, name="gradient"):
+    """-> the tensors, their device, how many, and as arrays for the C entry their addresses, sizes and type codes"""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise _lib.OgmmError("no %s tensors given" % name)
     dev = _dev("%s 0" % name, grads[0])
-    n = len(grads)
-    types = []
+    n, index = len(grads), dev.index
     for i, g in enumerate(grads):
-        c = _TYPE.get(g.dtype) if isinstance(g, torch.Tensor) and g.layout is torch.strided else None
-        if c is None or g.device != dev:
+        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.get_device() != index or g.dtype not in _TYPE:
             raise _lib.OgmmError("%s %d must be a dense float32, bfloat16 or float16 tensor on %s" % (name, i, dev))
-        if not _dense(g):
+        if not g.is_contiguous() and not _dense(g):
             raise _lib.OgmmError("%s %d has gaps or overlaps between its elements (shape %s, strides %s)" % (name, i, tuple(g.shape), g.stride()))
-        types.append(c)
-    return grads, dev, n, (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]), (ctypes.c_int32 * n)(*types)
+    # (bytes of an array are taken over in one piece; ctypes arrays convert value by value)
+    return (grads, dev, n, array.array("Q", [g.data_ptr() for g in grads]).tobytes(), array.array("q", [g.numel() for g in grads]).tobytes(),
+            array.array("i", [_TYPE[g.dtype] for g in grads]).tobytes())
 
 
 def grad_norm(grads, inv_scale=1.0):
@@ -1423,9 +1433,9 @@ def clip_grads_(grads, max_norm, inv_scale=1.0, out=None):
                 raise _lib.OgmmError("out %d must be a float32 tensor %s on %s" % (i, tuple(g.shape), dev))
             if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                 raise _lib.OgmmError("out %d must have the strides of its gradient" % i)
-            if not _dense(o):
+            if not o.is_contiguous() and not _dense(o):
                 raise _lib.OgmmError("out %d has gaps or overlaps between its elements (shape %s, strides %s)" % (i, tuple(o.shape), o.stride()))
-        outs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
+        outs = array.array("Q", [o.data_ptr() for o in out]).tobytes()
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(_lib.load().ogmm_grad_norm_workspace_bytes(n, numel), dtype=torch.uint8, device=dev)
     _call_on(dev, "ogmm_clip_grads", n, ptrs, numel, types, outs, inv_scale, max_norm, norm.data_ptr(), ws.data_ptr())

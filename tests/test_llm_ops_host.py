@@ -60,6 +60,10 @@ def test_struct_matches_the_header():
     body = header[header.index("typedef struct ogmm_xattn {"):header.index("} ogmm_xattn;")]
     fields = re.findall(r"[\*\s]([A-Za-z_0-9]+)\s*[;,]", re.sub(r"/\*.*?\*/", "", body, flags=re.S))
     assert fields == [f[0] for f in _lib.XattnDesc._fields_]
+    assert ops._XATTN.size == ctypes.sizeof(_lib.XattnDesc)
+    values = list(range(1, 36))
+    got = _lib.XattnDesc.from_buffer_copy(ops._XATTN.pack(*values))
+    assert [getattr(got, f) for f in fields] == values
 
 
 def norm_args(**kw):
