@@ -4,7 +4,7 @@
 //     dx = rstd (g - xh mean(g xh)) + dh,   dw = sum over rows of dy xh,
 // and its output in 8 bits: s = max|y| / 448 over the row or over each group of its columns, q = e4m3(y / s).
 //
-// Bound by HBM: a few operations for each value read or written.  A row is taken by 8, 64, 256 or 1024 lanes, so that a lane holds at most 32 values of it (one to
+// Bound by HBM: a few operations for each value read or written.  A row is taken by 8, 16, 32, 64, 256 or 1024 lanes, so that a lane holds at most 32 values of it (one to
 // eight loads of sixteen bytes, all in flight before the first is used) and the sum is one exchange inside a wave, or one through LDS.  The weights of a lane's
 // columns are read once and stay in registers for all the rows that its workgroup takes.  Rows may start anywhere (odd widths, strides): the part reads sixteen
 // bytes from any address; only a row's last, partial piece goes value by value.
@@ -35,6 +35,24 @@ __device__ __forceinline__ void load(const T* __restrict__ row, int c, int D, fl
 #pragma unroll
         for (int k = 0; k < N; ++k) out[k] = c + k < D ? static_cast<float>(row[c + k]) : 0.0f;
     }
+}
+
+// sixteen bytes as they lie in memory, to be widened when they are used: a wide row's values take half the registers
+struct Raw { uint32_t w[4]; };
+template <class T>
+__device__ __forceinline__ Raw fetch(const T* __restrict__ row, int c, int D) {
+    constexpr int N = 16 / sizeof(T);
+    if (c + N <= D) return __builtin_bit_cast(Raw, *reinterpret_cast<const Piece<T, N>*>(row + c));
+    Piece<T, N> p;
+#pragma unroll
+    for (int k = 0; k < N; ++k) p.v[k] = c + k < D ? row[c + k] : static_cast<T>(0.0f);
+    return __builtin_bit_cast(Raw, p);
+}
+template <class T>
+__device__ __forceinline__ float value(const Raw& r, int k) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[k]);
+    else if constexpr (std::is_same_v<T, __bf16>) return __uint_as_float(k & 1 ? r.w[k / 2] & 0xffff0000u : r.w[k / 2] << 16);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(k & 1 ? r.w[k / 2] >> 16 : r.w[k / 2] & 0xffff)));
 }
 
 template <int N, class T>
@@ -189,55 +207,85 @@ struct BwdArgs {
 };
 
 template <class T, class W, int LANES, int ITEMS>
-__global__ __launch_bounds__(THREADS<LANES>) void rms_norm_bwd_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(THREADS<LANES>, (LANES > 256 ? 4 : 2)) void rms_norm_bwd_kernel(const BwdArgs a) {
     constexpr int VEC = 16 / sizeof(T), PER = THREADS<LANES> / LANES;
     __shared__ float lds[2 * (LANES > 64 ? LANES / 64 : 1)];
     __shared__ float share[PER > 1 ? PER * LANES * VEC : 1];
     int slot = 0;
     const int lane = threadIdx.x % LANES, D = a.D;
-    float w[ITEMS][VEC], dw[ITEMS][VEC];
+    // the weights: in registers in 32 bits, or where 1024 lanes leave few of those in the rows' own 16
+    constexpr bool RAW_W = LANES > 256 && sizeof(W) == 2;
+    constexpr int WVEC = 16 / sizeof(W);
+    Raw w_raw[RAW_W ? ITEMS : 1];
+    float w[RAW_W ? 1 : ITEMS][VEC], dw[ITEMS][VEC];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        load<VEC>(static_cast<const W*>(a.w), (i * LANES + lane) * VEC, D, w[i]);
+        if constexpr (RAW_W) w_raw[i] = fetch<W>(static_cast<const W*>(a.w), (i * LANES + lane) * VEC, D);
+        else load<VEC>(static_cast<const W*>(a.w), (i * LANES + lane) * VEC, D, w[i]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) dw[i][k] = 0.0f;
     }
+    static_assert(!RAW_W || WVEC == VEC, "weights");
+    auto weight = [&](int i, int k) {
+        if constexpr (RAW_W) return value<W>(w_raw[i], k);
+        else return w[i][k];
+    };
     const float inv_d = 1.0f / D;
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * PER; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * PER) {
-        const int64_t row = row0 + threadIdx.x / LANES;
-        const bool here = LANES > 64 || row < a.rows;
-        const int d = here ? D : 0;
-        const T *dy = static_cast<const T*>(a.dy) + row * a.lddy, *h = static_cast<const T*>(a.h) + row * a.ldh;
-        const float rstd = here ? a.rstd[row] : 0.0f;
-        float g[ITEMS][VEC], xh[ITEMS][VEC];
+    // Where the registers allow it, the next row is on its way while this one is worked on
+    constexpr bool AHEAD = LANES <= 256;
+    Raw rg[ITEMS], rh[ITEMS], ru[ITEMS];
+    float rstd = 0.0f;
+    auto fetch_row = [&](Raw (&g)[ITEMS], Raw (&h)[ITEMS], Raw (&u)[ITEMS], float& r, int64_t row) {          // (a row's lanes agree on whether it is there)
+        const int d = row < a.rows ? D : 0;
+        r = d ? a.rstd[row] : 0.0f;
+        const T *pg = static_cast<const T*>(a.dy) + row * a.lddy, *ph = static_cast<const T*>(a.h) + row * a.ldh, *pu = static_cast<const T*>(a.dh) + row * a.lddh;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            load<VEC>(dy, (i * LANES + lane) * VEC, d, g[i]);
-            load<VEC>(h, (i * LANES + lane) * VEC, d, xh[i]);
+            g[i] = fetch<T>(pg, (i * LANES + lane) * VEC, d);
+            h[i] = fetch<T>(ph, (i * LANES + lane) * VEC, d);
+            if (a.dh) u[i] = fetch<T>(pu, (i * LANES + lane) * VEC, d);
         }
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * PER;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * PER + threadIdx.x / LANES;
+    if constexpr (AHEAD) fetch_row(rg, rh, ru, rstd, row);
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * PER; row0 < a.rows; row0 += step, row += step) {
+        if constexpr (!AHEAD) fetch_row(rg, rh, ru, rstd, row);
+        Raw ng[AHEAD ? ITEMS : 1], nh[AHEAD ? ITEMS : 1], nu[AHEAD ? ITEMS : 1];
+        float next_rstd = 0.0f;
+        if constexpr (AHEAD)
+            if (row0 + step < a.rows) fetch_row(ng, nh, nu, next_rstd, row + step);
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                xh[i][k] *= rstd;
-                dw[i][k] = fmaf(g[i][k], xh[i][k], dw[i][k]);
-                g[i][k] *= w[i][k];
-                dot = fmaf(g[i][k], xh[i][k], dot);
+                const float g = value<T>(rg[i], k), xh = value<T>(rh[i], k) * rstd;
+                dw[i][k] = fmaf(g, xh, dw[i][k]);
+                dot = fmaf(g * weight(i, k), xh, dot);
             }
         dot = over_row<LANES, false>(dot, lds, slot) * inv_d;
+        const int d = row < a.rows ? D : 0;
+        // (widened once more below: kept wide across the exchange, the row would take twice the registers)
+        if constexpr (sizeof(T) == 2)
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(rg[i].w[j]), "+v"(rh[i].w[j]));
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             float dx[VEC];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) dx[k] = rstd * (g[i][k] - xh[i][k] * dot);
-            if (a.dh) {
-                float u[VEC];
-                load<VEC>(static_cast<const T*>(a.dh) + row * a.lddh, (i * LANES + lane) * VEC, d, u);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) dx[k] += u[k];
+            for (int k = 0; k < VEC; ++k) {
+                dx[k] = rstd * (value<T>(rg[i], k) * weight(i, k) - value<T>(rh[i], k) * rstd * dot);
+                if (a.dh) dx[k] += value<T>(ru[i], k);
             }
             store<VEC>(static_cast<T*>(a.dx) + row * D, (i * LANES + lane) * VEC, d, dx);
+        }
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) { rg[i] = ng[i]; rh[i] = nh[i]; ru[i] = nu[i]; }
+            rstd = next_rstd;
         }
     }
     float* part = a.part + static_cast<int64_t>(blockIdx.x) * D;
@@ -287,7 +335,8 @@ int with_shape(int D, int least_lanes, F&& f) {
 #define OGMM_SHAPE(L, I) if (n <= L * I && least_lanes <= L) return go(integral_constant<int, L>(), integral_constant<int, I>())
     OGMM_SHAPE(8, 1);
     OGMM_SHAPE(8, 2);
-    OGMM_SHAPE(64, 1);
+    OGMM_SHAPE(16, 2);
+    OGMM_SHAPE(32, 2);
     OGMM_SHAPE(64, 2);
     OGMM_SHAPE(64, 4);
     OGMM_SHAPE(256, 2);
@@ -313,13 +362,14 @@ int launch_norm(const NormArgs& a, bool q8, hipStream_t stream) {
     });
 }
 
-constexpr int BWD_BLOCKS = 512;
+// dw's shares are written and read again (blocks x D x 4 bytes): two workgroups to a CU for wide rows, four for narrow ones, whose waves have fewer bytes on their way each
+constexpr int BWD_BLOCKS = 1024;
 
 template <class T, class W>
 int launch_bwd(const BwdArgs& a, void* dw, hipStream_t stream) {
     return with_shape<T>(a.D, 1, [&](auto lanes, auto items) {
         constexpr int L = decltype(lanes)::value, I = decltype(items)::value;
-        const int blocks = blocks_for(a.rows, THREADS<L> / L, BWD_BLOCKS);
+        const int blocks = blocks_for(a.rows, THREADS<L> / L, L > 64 ? BWD_BLOCKS / 2 : BWD_BLOCKS);
         if (blocks) rms_norm_bwd_kernel<T, W, L, I><<<blocks, THREADS<L>, 0, stream>>>(a);
         rms_norm_dw_kernel<W><<<(a.D + 63) / 64, 1024, 0, stream>>>(a.part, blocks, a.D, static_cast<W*>(dw));
         return check_launch("ogmm_rms_norm_bwd");

@@ -32,8 +32,6 @@ using InPlace = Table<230, false>;
 using OutOfPlace = Table<156, true>;
 static_assert(sizeof(InPlace) <= 4032 && sizeof(OutOfPlace) <= 4032, "kernel arguments");
 
-struct __attribute__((packed, aligned(2))) Bits16 { uint32_t w[4]; };          // sixteen bytes at an address of any alignment that the element has
-
 __device__ __forceinline__ float half_bits(uint32_t h, int type) {
     if (type == OGMM_BF16) return __uint_as_float(h << 16);
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
@@ -58,6 +56,26 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
     return s;
 }
 
+// bytes at an address of any alignment that the element has
+template <int BYTES> struct __attribute__((packed, aligned(2))) Packed { uint32_t w[BYTES / 4]; };
+
+// f(values, where) over a chunk's values, VEC to a thread at once and four loads in flight; f1(place) for the last few
+template <int BYTES, int VEC, class F, class F1>
+__device__ __forceinline__ void over_chunk(const char* __restrict__ p, uint32_t len, F&& f, F1&& f1) {
+    constexpr uint32_t ROUND = THREADS * VEC;
+    constexpr int E = BYTES / VEC;
+    uint32_t at = threadIdx.x * VEC;
+    for (; at + 3 * ROUND + VEC <= len; at += 4 * ROUND) {
+        Packed<BYTES> b[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) b[u] = *reinterpret_cast<const Packed<BYTES>*>(p + (at + u * ROUND) * E);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) f(b[u], at + u * ROUND);
+    }
+    for (; at + VEC <= len; at += ROUND) f(*reinterpret_cast<const Packed<BYTES>*>(p + at * E), at);
+    if (threadIdx.x < len % VEC) f1(len - len % VEC + threadIdx.x);
+}
+
 template <int N, bool OUT>
 __global__ __launch_bounds__(THREADS) void grad_squares_kernel(const Table<N, OUT> t, int n, uint32_t chunks, uint32_t chunk_len, double* __restrict__ partial) {
     __shared__ double lds[THREADS / 64];
@@ -67,27 +85,25 @@ __global__ __launch_bounds__(THREADS) void grad_squares_kernel(const Table<N, OU
         const uint32_t off = (c - t.first[i]) * chunk_len, len = min(chunk_len, t.count[i] - off);
         const int type = t.type[i];
         if (type == OGMM_F32) {
-            const float* __restrict__ p = static_cast<const float*>(t.g[i]) + off;
-#pragma unroll 4
-            for (uint32_t e = threadIdx.x * 4; e + 4 <= len; e += THREADS * 4) {
-                const Bits16 b = *reinterpret_cast<const Bits16*>(p + e);
+            const float* p = static_cast<const float*>(t.g[i]) + off;
+            over_chunk<16, 4>(reinterpret_cast<const char*>(p), len,
+                [&](const Packed<16>& b, uint32_t) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) { const double x = __uint_as_float(b.w[k]); acc = fma(x, x, acc); }
-            }
-            if (threadIdx.x < (len & 3)) { const double x = p[(len & ~3u) + threadIdx.x]; acc = fma(x, x, acc); }
+                    for (int k = 0; k < 4; ++k) { const double x = __uint_as_float(b.w[k]); acc = fma(x, x, acc); }
+                },
+                [&](uint32_t e) { const double x = p[e]; acc = fma(x, x, acc); });
         } else {
-            const uint16_t* __restrict__ p = static_cast<const uint16_t*>(t.g[i]) + off;
-#pragma unroll 2
-            for (uint32_t e = threadIdx.x * 8; e + 8 <= len; e += THREADS * 8) {
-                const Bits16 b = *reinterpret_cast<const Bits16*>(p + e);
+            const uint16_t* p = static_cast<const uint16_t*>(t.g[i]) + off;
+            over_chunk<16, 8>(reinterpret_cast<const char*>(p), len,
+                [&](const Packed<16>& b, uint32_t) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const double x = half_bits(b.w[k] & 0xffff, type), y = half_bits(b.w[k] >> 16, type);
-                    acc = fma(x, x, acc);
-                    acc = fma(y, y, acc);
-                }
-            }
-            if (threadIdx.x < (len & 7)) { const double x = half_bits(p[(len & ~7u) + threadIdx.x], type); acc = fma(x, x, acc); }
+                    for (int k = 0; k < 4; ++k) {
+                        const double x = half_bits(b.w[k] & 0xffff, type), y = half_bits(b.w[k] >> 16, type);
+                        acc = fma(x, x, acc);
+                        acc = fma(y, y, acc);
+                    }
+                },
+                [&](uint32_t e) { const double x = half_bits(p[e], type); acc = fma(x, x, acc); });
         }
     }
     const double s = block_sum(acc, lds);
@@ -123,47 +139,37 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(const Table<N, OUT> 
         if (type == OGMM_F32) {
             const float* p = static_cast<const float*>(t.g[i]) + off;
             float* o = OUT ? t.out[OUT ? i : 0] + off : static_cast<float*>(t.g[i]) + off;
-#pragma unroll 4
-            for (uint32_t e = threadIdx.x * 4; e + 4 <= len; e += THREADS * 4) {
-                Bits16 b = *reinterpret_cast<const Bits16*>(p + e);
+            over_chunk<16, 4>(reinterpret_cast<const char*>(p), len,
+                [&](Packed<16> b, uint32_t e) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) b.w[k] = __float_as_uint(__uint_as_float(b.w[k]) * f);
-                *reinterpret_cast<Bits16*>(o + e) = b;
-            }
-            if (threadIdx.x < (len & 3)) { const uint32_t e = (len & ~3u) + threadIdx.x; o[e] = p[e] * f; }
-        } else {
+                    for (int k = 0; k < 4; ++k) b.w[k] = __float_as_uint(__uint_as_float(b.w[k]) * f);
+                    *reinterpret_cast<Packed<16>*>(o + e) = b;
+                },
+                [&](uint32_t e) { o[e] = p[e] * f; });
+        } else if (OUT) {          // four values to a thread: its sixteen bytes of output lie beside its neighbours'
             const uint16_t* p = static_cast<const uint16_t*>(t.g[i]) + off;
-#pragma unroll 2
-            for (uint32_t e = threadIdx.x * 8; e + 8 <= len; e += THREADS * 8) {
-                const Bits16 b = *reinterpret_cast<const Bits16*>(p + e);
-                float x[8];
+            float* o = t.out[OUT ? i : 0] + off;
+            over_chunk<8, 4>(reinterpret_cast<const char*>(p), len,
+                [&](const Packed<8>& b, uint32_t e) {
+                    Packed<16> r;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[2 * k] = half_bits(b.w[k] & 0xffff, type) * f;
-                    x[2 * k + 1] = half_bits(b.w[k] >> 16, type) * f;
-                }
-                if (OUT) {
-                    float* o = t.out[OUT ? i : 0] + off + e;
-                    Bits16 r;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) r.w[k] = __float_as_uint(x[4 * h + k]);
-                        *reinterpret_cast<Bits16*>(o + 4 * h) = r;
+                    for (int k = 0; k < 2; ++k) {
+                        r.w[2 * k] = __float_as_uint(half_bits(b.w[k] & 0xffff, type) * f);
+                        r.w[2 * k + 1] = __float_as_uint(half_bits(b.w[k] >> 16, type) * f);
                     }
-                } else {
-                    Bits16 r;
+                    *reinterpret_cast<Packed<16>*>(o + e) = r;
+                },
+                [&](uint32_t e) { o[e] = half_bits(p[e], type) * f; });
+        } else {
+            uint16_t* p = static_cast<uint16_t*>(t.g[i]) + off;
+            over_chunk<16, 8>(reinterpret_cast<const char*>(p), len,
+                [&](Packed<16> b, uint32_t e) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) r.w[k] = to_half_bits(x[2 * k], type) | static_cast<uint32_t>(to_half_bits(x[2 * k + 1], type)) << 16;
-                    *reinterpret_cast<Bits16*>(static_cast<uint16_t*>(t.g[i]) + off + e) = r;
-                }
-            }
-            if (threadIdx.x < (len & 7)) {
-                const uint32_t e = (len & ~7u) + threadIdx.x;
-                const float x = half_bits(p[e], type) * f;
-                if (OUT) t.out[OUT ? i : 0][off + e] = x;
-                else (static_cast<uint16_t*>(t.g[i]) + off)[e] = to_half_bits(x, type);
-            }
+                    for (int k = 0; k < 4; ++k)
+                        b.w[k] = to_half_bits(half_bits(b.w[k] & 0xffff, type) * f, type) | static_cast<uint32_t>(to_half_bits(half_bits(b.w[k] >> 16, type) * f, type)) << 16;
+                    *reinterpret_cast<Packed<16>*>(p + e) = b;
+                },
+                [&](uint32_t e) { p[e] = to_half_bits(half_bits(p[e], type) * f, type); });
         }
     }
 }

@@ -4,6 +4,7 @@ stream and returns without synchronising.  All tensors must be CUDA (ROCm) tenso
 """
 import array
 import ctypes
+import operator
 import struct
 
 import torch
@@ -1172,6 +1173,7 @@ def weight_grad_thin(dy, x, split=False, overflow=None):
 
 # ---------------------------------------------------------------------------------------------- operators of large language models (csrc/cross_attention.hip, rms_norm.hip, train_clip.hip)
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # OGMM_F32 / OGMM_BF16 / OGMM_F16
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
 def _dev(name, first, **others):
@@ -1398,15 +1400,20 @@ def _grad_list(grads, name="gradient"):
     if not grads:
         raise _lib.OgmmError("no %s tensors given" % name)
     dev = _dev("%s 0" % name, grads[0])
-    n, index = len(grads), dev.index
-    for i, g in enumerate(grads):
-        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.get_device() != index or g.dtype not in _TYPE:
-            raise _lib.OgmmError("%s %d must be a dense float32, bfloat16 or float16 tensor on %s" % (name, i, dev))
-        if not g.is_contiguous() and not _dense(g):
-            raise _lib.OgmmError("%s %d has gaps or overlaps between its elements (shape %s, strides %s)" % (name, i, tuple(g.shape), g.stride()))
-    # (bytes of an array are taken over in one piece; ctypes arrays convert value by value)
-    return (grads, dev, n, array.array("Q", [g.data_ptr() for g in grads]).tobytes(), array.array("q", [g.numel() for g in grads]).tobytes(),
-            array.array("i", [_TYPE[g.dtype] for g in grads]).tobytes())
+    T = torch.Tensor
+    try:          # a hundred tensors and more at a call: checked and listed all at once, and one by one only to say which is wrong
+        types = array.array("i", map(_TYPE.__getitem__, map(_DTYPE_OF, grads)))
+        ptrs, numel = array.array("Q", map(T.data_ptr, grads)), array.array("q", map(T.numel, grads))
+        good = set(map(T.get_device, grads)) == {dev.index} and all(map(T.is_contiguous, grads))
+    except (KeyError, TypeError, AttributeError, RuntimeError):
+        good = False
+    if not good:
+        for i, g in enumerate(grads):
+            if not isinstance(g, T) or g.layout is not torch.strided or g.device != dev or g.dtype not in _TYPE:
+                raise _lib.OgmmError("%s %d must be a dense float32, bfloat16 or float16 tensor on %s" % (name, i, dev))
+            if not _dense(g):
+                raise _lib.OgmmError("%s %d has gaps or overlaps between its elements (shape %s, strides %s)" % (name, i, tuple(g.shape), g.stride()))
+    return grads, dev, len(grads), ptrs.tobytes(), numel.tobytes(), types.tobytes()          # (an array's bytes are taken over in one piece by the C entry)
 
 
 def grad_norm(grads, inv_scale=1.0):
