@@ -40,6 +40,18 @@ __device__ __forceinline__ uint32_t item_of(const Args& a) {
     return (at / a.run * 8 + xcd) * a.run + at % a.run;
 }
 
+// The batch entry that comes b-th: where lengths differ the longest first, so that the last workgroups to start are the shortest (up to 64 entries: a lane ranks one)
+__device__ __forceinline__ int batch_of(const Args& a, int b) {
+    if (!a.kv_lens || a.B > 64 || a.B == 1) return b;
+    const int lane = threadIdx.x & 63, mine = lane < a.B ? clamp_len(a.kv_lens, lane, a.Nk) : -1;
+    int rank = 0;
+    for (int i = 0; i < a.B; ++i) {
+        const int other = __builtin_amdgcn_readlane(mine, i);
+        rank += other > mine || (other == mine && i < lane);
+    }
+    return __ffsll(static_cast<unsigned long long>(__ballot(lane < a.B && rank == b))) - 1;
+}
+
 // ---- products of 32x32 tiles, sixteen bytes of either operand to a lane: row lane % 32, byte 16 (lane / 32) of a 32-byte chunk of the contraction
 __device__ __forceinline__ void mma(f32x16& c, u32x4 a, u32x4 b, __bf16) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -283,7 +295,8 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int split = item % a.splits, tile = item / a.splits % a.tiles, bh = item / a.splits / a.tiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int split = item % a.splits, tile = item / a.splits % a.tiles, of = item / a.splits / a.tiles, hk = of % a.Hkv, b = batch_of(a, of / a.Hkv), bh = b * a.Hkv + hk;
+    const int64_t place = (static_cast<int64_t>(bh) * a.tiles + tile) * a.splits + split;          // of its part
     const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
     const char *k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h);
     const char *v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h);
@@ -409,7 +422,7 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
         if (out_row < a.rows) {
             const int on = out_row / a.G, og = out_row - on * a.G;
             const float inv = a.splits > 1 ? 1.0f : all.y > 0.0f ? 1.0f / all.y : all.y;
-            float* part = a.splits > 1 ? a.part + (static_cast<int64_t>(item) * 32 + r) * a.d : nullptr;
+            float* part = a.splits > 1 ? a.part + (place * 32 + r) * a.d : nullptr;
             const int64_t out = ((static_cast<int64_t>(b) * a.Nq + on) * a.H + hk * a.G + og) * a.d;
             for (int ch = threadIdx.x & 7; ch < a.d; ch += 8) {
                 float x = 0.0f;
@@ -419,15 +432,15 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
                 else store_one<T>(a, out + ch, x * inv);
             }
             if ((threadIdx.x & 7) == 0) {
-                if (a.splits > 1) reinterpret_cast<float2*>(a.part_ml)[static_cast<int64_t>(item) * 32 + r] = all;
+                if (a.splits > 1) reinterpret_cast<float2*>(a.part_ml)[place * 32 + r] = all;
                 else if (a.lse) a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + og) * a.Nq + on] = all.y == 0.0f ? -INFINITY : (all.x + log2f(all.y)) * LN2;
             }
         }
     } else {
         if (row >= a.rows) return;
         if (a.splits > 1) {
-            if (lane < 32) reinterpret_cast<float2*>(a.part_ml)[static_cast<int64_t>(item) * S::ROWS + wave * 32 + lane] = make_float2(m, l);
-            store_part<M>(a.part + (static_cast<int64_t>(item) * S::ROWS + wave * 32 + (lane & 31)) * a.d, o, 1.0f, a.d);
+            if (lane < 32) reinterpret_cast<float2*>(a.part_ml)[place * S::ROWS + wave * 32 + lane] = make_float2(m, l);
+            store_part<M>(a.part + (place * S::ROWS + wave * 32 + (lane & 31)) * a.d, o, 1.0f, a.d);
             return;
         }
         const int64_t out = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
@@ -555,7 +568,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 1
     const uint32_t item = item_of(a);
     if (item >= a.items) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int split = item % a.row_splits, tile = item / a.row_splits % a.row_tiles, bh = item / a.row_splits / a.row_tiles, hk = bh % a.Hkv, b = bh / a.Hkv;
+    const int split = item % a.row_splits, tile = item / a.row_splits % a.row_tiles, of = item / a.row_splits / a.row_tiles, hk = of % a.Hkv, b = batch_of(a, of / a.Hkv), bh = b * a.Hkv + hk;
     const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
     const char *k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h);
     const char *v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h);
