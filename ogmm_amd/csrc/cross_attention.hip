@@ -458,18 +458,21 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a, int tile_
     const int row = w % a.rows, bh = w / a.rows, hk = bh % a.Hkv, b = bh / a.Hkv, tile = row / tile_rows, n = row / a.G, g = row - n * a.G;
     const int64_t first = (static_cast<int64_t>(bh) * a.tiles + tile) * a.splits;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+    const int64_t at0 = first * tile_rows + row % tile_rows;          // part s: tile_rows rows further on for each
     float top = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[(first + s) * tile_rows + row % tile_rows].x);
+    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[at0 + s * tile_rows].x);
     top = wave_max(top);
+    if (top == -INFINITY) top = 0.0f;          // (no key at all: every part is zero)
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t at = (first + s) * tile_rows + row % tile_rows;
+    const int c0 = min(lane, a.d - 1), c1 = min(lane + 64, a.d - 1);
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {          // (every part is written, an empty one as zeros: the loads need not wait for each other)
+        const int64_t at = at0 + s * tile_rows;
         const float2 x = ml[at];
-        if (x.x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(x.x - top);
+        const float u0 = a.part[at * a.d + c0], u1 = a.part[at * a.d + c1], f = __builtin_amdgcn_exp2f(x.x - top);
         l = fmaf(x.y, f, l);
-        if (lane < a.d) o0 = fmaf(a.part[at * a.d + lane], f, o0);
-        if (lane + 64 < a.d) o1 = fmaf(a.part[at * a.d + lane + 64], f, o1);
+        o0 = fmaf(u0, f, o0);
+        o1 = fmaf(u1, f, o1);
     }
     const float inv = l > 0.0f ? 1.0f / l : l;
     const int64_t out = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;

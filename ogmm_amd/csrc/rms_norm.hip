@@ -369,7 +369,7 @@ template <class T, class W>
 int launch_bwd(const BwdArgs& a, void* dw, hipStream_t stream) {
     return with_shape<T>(a.D, 1, [&](auto lanes, auto items) {
         constexpr int L = decltype(lanes)::value, I = decltype(items)::value;
-        const int blocks = blocks_for(a.rows, THREADS<L> / L, L > 64 ? BWD_BLOCKS / 2 : BWD_BLOCKS);
+        const int blocks = blocks_for(a.rows, THREADS<L> / L, L > 32 ? BWD_BLOCKS / 2 : BWD_BLOCKS);
         if (blocks) rms_norm_bwd_kernel<T, W, L, I><<<blocks, THREADS<L>, 0, stream>>>(a);
         rms_norm_dw_kernel<W><<<(a.D + 63) / 64, 1024, 0, stream>>>(a.part, blocks, a.D, static_cast<W*>(dw));
         return check_launch("ogmm_rms_norm_bwd");

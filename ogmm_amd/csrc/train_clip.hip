@@ -1,9 +1,9 @@
 // Global norm of many gradient tensors, and their clipping:  n = inv_scale sqrt(sum g^2),  c = min(1, max_norm / (n + 1e-6)),  out = g * (inv_scale c).
 //
 // Bound by HBM: every value is read once for the norm, and read and written once more where the factor is not one.  The tensors travel as a table in the
-// kernel arguments (no copy, nothing kept between calls, capturable); they are cut into chunks that the workgroups of one launch take in turn, so a hundred
-// small tensors fill the part as well as one large one.  Squares are formed and summed in fp64 from the first value on: fp32 squares of gradients below 1e-19
-// or above 1e19 leave its range, and the fp64 FMA rate is several times what the stream of values needs.  Every sum has a fixed order: results repeat bit for bit.
+// kernel arguments (no copy, nothing kept between calls, capturable); each workgroup takes an equal run of their values, so a hundred small tensors
+// fill the part as well as one large one.  Squares are summed in fp64: four or eight of them in fp32 first, where
+// that is inside its range.  Every sum has a fixed order: results repeat bit for bit.
 #include "ogmm_common.h"
 #include <algorithm>
 #include <exception>
@@ -17,6 +17,7 @@ using namespace ogmm;
 constexpr int THREADS = 1024;
 // 512 workgroups of 1024 threads are all the waves that the 256 CUs hold; with one partial sum each the second kernel can add them up by itself in every workgroup
 constexpr int MAX_BLOCKS = 512;
+constexpr uint32_t CHUNK = 4096;            // what the work is dealt in: a load of sixteen bytes for each thread (fp32)
 constexpr int64_t PIECE = 1 << 30;          // a longer tensor goes into the table as several pieces, so that sizes fit 32 bits
 
 // A launch's tensors; the kernel argument segment is 4 KB: 230 tensors by one address, or 156 by two (out of place)
@@ -37,14 +38,25 @@ __device__ __forceinline__ float half_bits(uint32_t h, int type) {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
 }
 
-template <int N, bool OUT>
-__device__ __forceinline__ int tensor_of(const Table<N, OUT>& t, int n, uint32_t chunk) {
-    int lo = 0, hi = n - 1;          // the last tensor whose first chunk is not behind `chunk` (empty tensors share it with their successor)
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+// Workgroups take runs of `run` chunks in turn (few tensors: one run each): f(tensor, first value, how many) for each tensor that a run touches
+template <int N, bool OUT, class F>
+__device__ __forceinline__ void over_runs(const Table<N, OUT>& t, int n, uint32_t run, F&& f) {
+    const uint32_t chunks = t.first[n];
+    int lo = 0;
+    for (uint32_t c = blockIdx.x * run; c < chunks; c += (gridDim.x - 1) * run) {
+        const uint32_t end = min(c + run, chunks);
+        for (int hi = n - 1; lo < hi;) {          // the last tensor whose first chunk is not behind c
+            const int mid = (lo + hi + 1) >> 1;
+            if (t.first[mid] <= c) lo = mid; else hi = mid - 1;
+        }
+        for (;; ++lo) {
+            const uint32_t stop = min(end, t.first[lo + 1]), off = (c - t.first[lo]) * CHUNK;
+            f(lo, off, min((stop - c) * CHUNK, t.count[lo] - off));
+            c = stop;
+            if (c >= end) break;
+        }
+        if (end == chunks) break;
     }
-    return lo;
 }
 
 __device__ __forceinline__ double block_sum(double v, double* lds) {
@@ -59,53 +71,67 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 // bytes at an address of any alignment that the element has
 template <int BYTES> struct __attribute__((packed, aligned(2))) Packed { uint32_t w[BYTES / 4]; };
 
-// f(values, where) over a chunk's values, VEC to a thread at once and four loads in flight; f1(place) for the last few
-template <int BYTES, int VEC, class F, class F1>
-__device__ __forceinline__ void over_chunk(const char* __restrict__ p, uint32_t len, F&& f, F1&& f1) {
+// f(values, where) over a run's values, VEC to a thread at once and AHEAD loads in flight; f1(place) for single ones: those in front of the first place at which `by` (the run's first
+// value as it is read or written) is aligned to VEC values of its own, and the last few.  A tensor may start anywhere in a bucket, and loads that straddle lines take half as long again.
+template <int BYTES, int VEC, int AHEAD, class P, class F, class F1>
+__device__ __forceinline__ void over_values(const char* __restrict__ p, const P* by, uint32_t len, F&& f, F1&& f1) {
     constexpr uint32_t ROUND = THREADS * VEC;
     constexpr int E = BYTES / VEC;
-    uint32_t at = threadIdx.x * VEC;
-    for (; at + 3 * ROUND + VEC <= len; at += 4 * ROUND) {
-        Packed<BYTES> b[4];
+    const uint32_t lead = min(len, static_cast<uint32_t>(-(reinterpret_cast<uintptr_t>(by) / sizeof(P)) % VEC)), tail = (len - lead) % VEC;
+    uint32_t at = lead + threadIdx.x * VEC;
+    for (; at + (AHEAD - 1) * ROUND + VEC <= len; at += AHEAD * ROUND) {
+        Packed<BYTES> b[AHEAD];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) b[u] = *reinterpret_cast<const Packed<BYTES>*>(p + (at + u * ROUND) * E);
+        for (int u = 0; u < AHEAD; ++u) b[u] = *reinterpret_cast<const Packed<BYTES>*>(p + static_cast<size_t>(at + u * ROUND) * E);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) f(b[u], at + u * ROUND);
+        for (int u = 0; u < AHEAD; ++u) f(b[u], at + u * ROUND);
     }
-    for (; at + VEC <= len; at += ROUND) f(*reinterpret_cast<const Packed<BYTES>*>(p + at * E), at);
-    if (threadIdx.x < len % VEC) f1(len - len % VEC + threadIdx.x);
+    for (; at + VEC <= len; at += ROUND) f(*reinterpret_cast<const Packed<BYTES>*>(p + static_cast<size_t>(at) * E), at);
+    if (threadIdx.x < lead) f1(threadIdx.x);
+    if (threadIdx.x < tail) f1(len - tail + threadIdx.x);
+}
+
+// acc += the squares of N values.  They are added up in fp32 first, where their sum stands well inside its range (their roundings are of random sign, 2^-24 at most); a group outside
+// it -- 1e-19 and 1e19 are the roots -- is formed in fp64.  A conversion to fp64 and its multiplication take six times an fp32 one.
+template <int N>
+__device__ __forceinline__ void add_squares(double& acc, const float (&x)[N]) {
+    float s = x[0] * x[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) s = fmaf(x[k], x[k], s);
+    if (s > 1e-30f && s < 1e30f) {
+        acc += s;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc = fma(static_cast<double>(x[k]), static_cast<double>(x[k]), acc);
+    }
 }
 
 template <int N, bool OUT>
-__global__ __launch_bounds__(THREADS) void grad_squares_kernel(const Table<N, OUT> t, int n, uint32_t chunks, uint32_t chunk_len, double* __restrict__ partial) {
+__global__ __launch_bounds__(THREADS, 8) void grad_squares_kernel(const Table<N, OUT> t, int n, uint32_t run, double* __restrict__ partial) {
     __shared__ double lds[THREADS / 64];
     double acc = 0.0;
-    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int i = tensor_of(t, n, c);
-        const uint32_t off = (c - t.first[i]) * chunk_len, len = min(chunk_len, t.count[i] - off);
+    over_runs(t, n, run, [&](int i, uint32_t off, uint32_t len) {
         const int type = t.type[i];
         if (type == OGMM_F32) {
             const float* p = static_cast<const float*>(t.g[i]) + off;
-            over_chunk<16, 4>(reinterpret_cast<const char*>(p), len,
+            over_values<16, 4, 4>(reinterpret_cast<const char*>(p), p, len,
                 [&](const Packed<16>& b, uint32_t) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) { const double x = __uint_as_float(b.w[k]); acc = fma(x, x, acc); }
+                    const float x[4] = {__uint_as_float(b.w[0]), __uint_as_float(b.w[1]), __uint_as_float(b.w[2]), __uint_as_float(b.w[3])};
+                    add_squares(acc, x);
                 },
                 [&](uint32_t e) { const double x = p[e]; acc = fma(x, x, acc); });
         } else {
             const uint16_t* p = static_cast<const uint16_t*>(t.g[i]) + off;
-            over_chunk<16, 8>(reinterpret_cast<const char*>(p), len,
+            over_values<16, 8, 4>(reinterpret_cast<const char*>(p), p, len,
                 [&](const Packed<16>& b, uint32_t) {
+                    float x[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const double x = half_bits(b.w[k] & 0xffff, type), y = half_bits(b.w[k] >> 16, type);
-                        acc = fma(x, x, acc);
-                        acc = fma(y, y, acc);
-                    }
+                    for (int k = 0; k < 4; ++k) { x[2 * k] = half_bits(b.w[k] & 0xffff, type); x[2 * k + 1] = half_bits(b.w[k] >> 16, type); }
+                    add_squares(acc, x);
                 },
                 [&](uint32_t e) { const double x = half_bits(p[e], type); acc = fma(x, x, acc); });
         }
-    }
+    });
     const double s = block_sum(acc, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -123,8 +149,8 @@ __global__ __launch_bounds__(THREADS) void grad_norm_finish_kernel(const double*
 }
 
 template <int N, bool OUT>
-__global__ __launch_bounds__(THREADS) void grad_clip_kernel(const Table<N, OUT> t, int n, uint32_t chunks, uint32_t chunk_len, const double* __restrict__ partial,
-                                                            int partials, double inv_scale, double max_norm, float* __restrict__ norm) {
+__global__ __launch_bounds__(THREADS, 8) void grad_clip_kernel(const Table<N, OUT> t, int n, uint32_t run, const double* __restrict__ partial, int partials, double inv_scale, double max_norm,
+                                                            float* __restrict__ norm) {
     __shared__ double lds[THREADS / 64];
     const double total = norm_of(partial, partials, inv_scale, lds);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(total);
@@ -132,14 +158,12 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(const Table<N, OUT> 
     if (c > 1.0) c = 1.0;          // (a NaN stays one: the gradients become NaN as they do in a plain product)
     const float f = static_cast<float>(c * inv_scale);
     if (!OUT && f == 1.0f) return;          // nothing changes
-    for (uint32_t ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
-        const int i = tensor_of(t, n, ch);
-        const uint32_t off = (ch - t.first[i]) * chunk_len, len = min(chunk_len, t.count[i] - off);
+    over_runs(t, n, run, [&](int i, uint32_t off, uint32_t len) {
         const int type = t.type[i];
         if (type == OGMM_F32) {
             const float* p = static_cast<const float*>(t.g[i]) + off;
             float* o = OUT ? t.out[OUT ? i : 0] + off : static_cast<float*>(t.g[i]) + off;
-            over_chunk<16, 4>(reinterpret_cast<const char*>(p), len,
+            over_values<16, 4, 4>(reinterpret_cast<const char*>(p), o, len,
                 [&](Packed<16> b, uint32_t e) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) b.w[k] = __float_as_uint(__uint_as_float(b.w[k]) * f);
@@ -149,7 +173,7 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(const Table<N, OUT> 
         } else if (OUT) {          // four values to a thread: its sixteen bytes of output lie beside its neighbours'
             const uint16_t* p = static_cast<const uint16_t*>(t.g[i]) + off;
             float* o = t.out[OUT ? i : 0] + off;
-            over_chunk<8, 4>(reinterpret_cast<const char*>(p), len,
+            over_values<8, 4, 8>(reinterpret_cast<const char*>(p), o, len,
                 [&](const Packed<8>& b, uint32_t e) {
                     Packed<16> r;
 #pragma unroll
@@ -162,7 +186,7 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(const Table<N, OUT> 
                 [&](uint32_t e) { o[e] = half_bits(p[e], type) * f; });
         } else {
             uint16_t* p = static_cast<uint16_t*>(t.g[i]) + off;
-            over_chunk<16, 8>(reinterpret_cast<const char*>(p), len,
+            over_values<16, 8, 4>(reinterpret_cast<const char*>(p), p, len,
                 [&](Packed<16> b, uint32_t e) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -171,7 +195,7 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(const Table<N, OUT> 
                 },
                 [&](uint32_t e) { p[e] = to_half_bits(half_bits(p[e], type) * f, type); });
         }
-    }
+    });
 }
 
 struct Item { void* g; float* out; uint32_t count; uint8_t type; };
@@ -221,15 +245,8 @@ void pieces_of(int n, const void* const* grads, const int64_t* numel, const int3
                              static_cast<uint32_t>(std::min(PIECE, numel[i] - at)), static_cast<uint8_t>(types[i])});
 }
 
-// Chunks so large that a workgroup takes about eight of them, within 4096 values (one load of sixteen bytes a thread) and 32768
-uint32_t chunk_length(int64_t total) {
-    uint32_t len = 4096;
-    while (len < 32768 && total > static_cast<int64_t>(len) * MAX_BLOCKS * 8) len *= 2;
-    return len;
-}
-
 template <class T, bool OUT>
-int fill(T& t, const std::vector<Item>& items, size_t from, uint32_t len, uint32_t* chunks) {
+int fill(T& t, const std::vector<Item>& items, size_t from) {
     constexpr size_t cap = sizeof(t.count) / sizeof(t.count[0]);
     const int n = static_cast<int>(std::min(cap, items.size() - from));
     uint32_t at = 0;
@@ -240,40 +257,40 @@ int fill(T& t, const std::vector<Item>& items, size_t from, uint32_t len, uint32
         t.count[k] = it.count;
         t.type[k] = it.type;
         t.first[k] = at;
-        at += (it.count + len - 1) / len;
+        at += (it.count + CHUNK - 1) / CHUNK;
     }
     t.first[n] = at;
-    *chunks = at;
     return n;
 }
 
-int64_t total_of(const std::vector<Item>& items) {
-    int64_t s = 0;
-    for (const Item& it : items) s += it.count;
-    return s;
+// How `chunks` are dealt: equal runs, one to a workgroup as long as that is 16 chunks or less.  (13 M values of 150 tensors: one run each 13.7 us, single chunks in turn 19; 300 M: runs
+// of 65536 values keep the workgroups' reads closer together than one run each would)
+struct Deal { int blocks; uint32_t run; };
+Deal deal(uint32_t chunks) {
+    const uint32_t rounds = std::max<uint32_t>(1, (chunks + 16 * MAX_BLOCKS - 1) / (16 * MAX_BLOCKS)), run = std::max<uint32_t>(1, (chunks + MAX_BLOCKS * rounds - 1) / (MAX_BLOCKS * rounds));
+    return {static_cast<int>(std::min<uint32_t>((chunks + run - 1) / run, MAX_BLOCKS)), run};
 }
 
-int launch_squares(const std::vector<Item>& items, uint32_t len, double* partial, int* partials, hipStream_t stream) {
+int launch_squares(const std::vector<Item>& items, double* partial, int* partials, hipStream_t stream) {
     *partials = 0;
     for (size_t from = 0; from < items.size();) {
         InPlace t;
-        uint32_t chunks;
-        const int n = fill<InPlace, false>(t, items, from, len, &chunks);
-        const int blocks = static_cast<int>(std::min<uint32_t>(chunks, MAX_BLOCKS));
-        grad_squares_kernel<<<blocks, THREADS, 0, stream>>>(t, n, chunks, len, partial + *partials);
-        *partials += blocks;
+        const int n = fill<InPlace, false>(t, items, from);
+        const Deal d = deal(t.first[n]);
+        grad_squares_kernel<<<d.blocks, THREADS, 0, stream>>>(t, n, d.run, partial + *partials);
+        *partials += d.blocks;
         from += n;
     }
     return check_launch("ogmm_grad_norm");
 }
 
 template <class T, bool OUT>
-void launch_clip(const std::vector<Item>& items, uint32_t len, const double* partial, int partials, double inv_scale, double max_norm, float* norm, hipStream_t stream) {
+void launch_clip(const std::vector<Item>& items, const double* partial, int partials, double inv_scale, double max_norm, float* norm, hipStream_t stream) {
     for (size_t from = 0; from < items.size();) {
         T t;
-        uint32_t chunks;
-        const int n = fill<T, OUT>(t, items, from, len, &chunks);
-        grad_clip_kernel<<<std::min<uint32_t>(chunks, MAX_BLOCKS), THREADS, 0, stream>>>(t, n, chunks, len, partial, partials, inv_scale, max_norm, from ? nullptr : norm);
+        const int n = fill<T, OUT>(t, items, from);
+        const Deal d = deal(t.first[n]);
+        grad_clip_kernel<<<d.blocks, THREADS, 0, stream>>>(t, n, d.run, partial, partials, inv_scale, max_norm, from ? nullptr : norm);
         from += n;
     }
 }
@@ -306,7 +323,7 @@ extern "C" int ogmm_grad_norm(int n, const void* const* grads, const int64_t* nu
         pieces_of(n, grads, numel, types, nullptr, items);
         int partials;
         double* partial = static_cast<double*>(workspace);
-        if (launch_squares(items, chunk_length(total_of(items)), partial, &partials, as_stream(stream))) return 1;
+        if (launch_squares(items, partial, &partials, as_stream(stream))) return 1;
         grad_norm_finish_kernel<<<1, THREADS, 0, as_stream(stream)>>>(partial, partials, inv_scale, norm);
         return check_launch("ogmm_grad_norm");
     });
@@ -324,16 +341,15 @@ extern "C" int ogmm_clip_grads(int n, const void* const* grads, const int64_t* n
         if (check_apart("ogmm_clip_grads", n, grads, numel, types, out)) return 1;
         std::vector<Item> items;
         pieces_of(n, grads, numel, types, out, items);
-        const uint32_t len = chunk_length(total_of(items));
         int partials;
         double* partial = static_cast<double*>(workspace);
-        if (launch_squares(items, len, partial, &partials, as_stream(stream))) return 1;
+        if (launch_squares(items, partial, &partials, as_stream(stream))) return 1;
         if (items.empty())
             grad_norm_finish_kernel<<<1, THREADS, 0, as_stream(stream)>>>(partial, 0, inv_scale, norm);
         else if (out)
-            launch_clip<OutOfPlace, true>(items, len, partial, partials, inv_scale, max_norm, norm, as_stream(stream));
+            launch_clip<OutOfPlace, true>(items, partial, partials, inv_scale, max_norm, norm, as_stream(stream));
         else
-            launch_clip<InPlace, false>(items, len, partial, partials, inv_scale, max_norm, norm, as_stream(stream));
+            launch_clip<InPlace, false>(items, partial, partials, inv_scale, max_norm, norm, as_stream(stream));
         return check_launch("ogmm_clip_grads");
     });
 }

@@ -1319,68 +1319,66 @@ def _rows(t, D):
 
 
 def _norm_args(x, weight, residual):
+    """-> device, type codes of rows and weight, D, weight, the rows of x and residual as (view, row stride)"""
     dev = _dev("x", x, weight=weight, residual=residual)
-    code = _code(x, "x")
+    code, wcode = _TYPE.get(x.dtype), _TYPE.get(weight.dtype)
+    if code is None:
+        _code(x, "x")
     shape = x.shape
     if not shape or not shape[-1] or weight.shape != shape[-1:]:
         raise _lib.OgmmError("weight must have one value for each of the last axis of x %s, got %s" % (tuple(shape), tuple(weight.shape)))
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+    if wcode != code and wcode != 0:
         raise _lib.OgmmError("weight must be %s or float32, got %s" % (x.dtype, weight.dtype))
-    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
-        raise _lib.OgmmError("residual must be %s %s, got %s %s" % (x.dtype, tuple(shape), residual.dtype, tuple(residual.shape)))
-    return dev, code, weight.contiguous()
+    D = shape[-1]
+    r = (None, 0)
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != x.dtype:
+            raise _lib.OgmmError("residual must be %s %s, got %s %s" % (x.dtype, tuple(shape), residual.dtype, tuple(residual.shape)))
+        r = _rows(residual, D)
+    return dev, code, wcode, D, weight.contiguous(), _rows(x, D), r
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight over the last axis (up to 32768 values).  x [..., D] float32, bfloat16 or float16 (rows with any stride);
     weight [D] of x's type or float32.  -> (y, h, rstd): h = x itself without a residual, otherwise the sum rounded to x's type (y is formed from the sum before
     that rounding); rstd fp32, one value a row, is what rms_norm_bwd() takes."""
-    dev, code, w = _norm_args(x, weight, residual)
-    D = x.shape[-1]
-    x2, ldx = _rows(x, D)
-    r2, ldr = _rows(residual, D) if residual is not None else (None, 0)
+    dev, code, wcode, D, w, (x2, ldx), (r2, ldr) = _norm_args(x, weight, residual)
     y = x.new_empty(x.shape)
-    h = x if residual is None else x.new_empty(x.shape)
+    h = x if r2 is None else x.new_empty(x.shape)
     rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    _call_on(dev, "ogmm_rms_norm", x2.data_ptr(), ldx, _ptr(r2), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps,
-             y.data_ptr(), None if residual is None else h.data_ptr(), rstd.data_ptr())
+    _call_on(dev, "ogmm_rms_norm", x2.data_ptr(), ldx, _ptr(r2), ldr, w.data_ptr(), x2.shape[0], D, code, wcode, eps, y.data_ptr(), 0 if r2 is None else h.data_ptr(), rstd.data_ptr())
     return y, h, rstd
 
 
 def rms_norm_q8(x, weight, residual=None, eps=1e-6, group=0):
     """rms_norm() with y in 8 bits: -> (q float8_e4m3fn [..., D], scales fp32, h); y = q * scale.  One scale a row (group = 0: scales [..., 1]) or one for each `group` = 32, 64 or
     128 columns (scales [..., ceil(D / group)]), the largest magnitude over 448."""
-    dev, code, w = _norm_args(x, weight, residual)
+    dev, code, wcode, D, w, (x2, ldx), (r2, ldr) = _norm_args(x, weight, residual)
     if group not in (0, 32, 64, 128):
         raise _lib.OgmmError("group must be 0 (one scale a row), 32, 64 or 128 columns, got %r" % (group,))
-    D = x.shape[-1]
-    x2, ldx = _rows(x, D)
-    r2, ldr = _rows(residual, D) if residual is not None else (None, 0)
     q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
-    scales = torch.empty(x.shape[:-1] + (-(-D // group) if group else 1,), dtype=torch.float32, device=dev)
-    h = x if residual is None else x.new_empty(x.shape)
-    _call_on(dev, "ogmm_rms_norm_q8", x2.data_ptr(), ldx, _ptr(r2), ldr, w.data_ptr(), x2.shape[0], D, code, _TYPE[w.dtype], eps, group,
-             q.data_ptr(), scales.data_ptr(), None if residual is None else h.data_ptr())
+    scales = x.new_empty(x.shape[:-1] + (-(-D // group) if group else 1,), dtype=torch.float32)
+    h = x if r2 is None else x.new_empty(x.shape)
+    _call_on(dev, "ogmm_rms_norm_q8", x2.data_ptr(), ldx, _ptr(r2), ldr, w.data_ptr(), x2.shape[0], D, code, wcode, eps, group, q.data_ptr(), scales.data_ptr(),
+             0 if r2 is None else h.data_ptr())
     return q, scales, h
 
 
 def rms_norm_bwd(dy, h, weight, rstd, dh=None):
     """Backward of rms_norm(): (dx, dweight) from dy = dL/dy, the forward's h and rstd, and dh = dL/dh where the sum has readers of its own; dx is the residual's gradient too."""
-    dev, code, w = _norm_args(h, weight, None)
+    dev, code, wcode, D, w, (h2, ldh), _ = _norm_args(h, weight, None)
     _dev("h", h, dy=dy, rstd=rstd, dh=dh)
     for n, t in (("dy", dy), ("dh", dh)):
         if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
             raise _lib.OgmmError("%s must be %s %s, got %s %s" % (n, h.dtype, tuple(h.shape), t.dtype, tuple(t.shape)))
     if _f32(rstd, "rstd").shape != h.shape[:-1]:
         raise _lib.OgmmError("rstd must have one value for each row of h %s, got %s" % (tuple(h.shape), tuple(rstd.shape)))
-    D = h.shape[-1]
-    (dy2, lddy), (h2, ldh), rstd = _rows(dy, D), _rows(h, D), rstd.contiguous()
+    (dy2, lddy), rstd = _rows(dy, D), rstd.contiguous()
     dh2, lddh = _rows(dh, D) if dh is not None else (None, 0)
     dx = h.new_empty(h.shape)
     dw = w.new_empty(D)
     ws = torch.empty(_lib.load().ogmm_rms_norm_bwd_workspace_bytes(h2.shape[0], D), dtype=torch.uint8, device=dev)
-    _call_on(dev, "ogmm_rms_norm_bwd", dy2.data_ptr(), lddy, h2.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), None if dh2 is None else dh2.data_ptr(), lddh, h2.shape[0], D,
-             code, _TYPE[w.dtype], dx.data_ptr(), dw.data_ptr(), ws.data_ptr())
+    _call_on(dev, "ogmm_rms_norm_bwd", dy2.data_ptr(), lddy, h2.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), _ptr(dh2), lddh, h2.shape[0], D, code, wcode, dx.data_ptr(), dw.data_ptr(), ws.data_ptr())
     return dx, dw
 
 
