@@ -540,7 +540,7 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(const BwdArgs a) {
 }
 
 // dS as an fp16 operand: times a power of two that brings the largest |dO| of the rows that share a key head to [1, 2), so that a gradient of any size keeps its precision
-// where fp16's exponents end (fp32 and bf16 have the range)
+// where fp16's exponents end (fp32 and bf16 have the range).  |P (dP - delta)| is half of max |dP| at most: nothing overflows while a key's |v| sum to 65504 or less.
 template <class T>
 __device__ __forceinline__ float gradient_scale(const BwdArgs& a, int bh) {
     if constexpr (std::is_same_v<T, _Float16>) {
@@ -959,8 +959,10 @@ int check(const char* who, const ogmm_xattn* a) {
     OGMM_REQUIRE(steps_fit(a, a->q_n, a->q_h) && steps_fit(a, a->k_n, 0) && steps_fit(a, a->v_n, 0), "%s: rows or heads are too far apart (32 MB and more)", who);
     OGMM_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->rest), "%s: addresses must be multiples of 16 bytes", who);
     OGMM_REQUIRE(isfinite(a->scale), "%s: scale must be finite", who);
-    // (a workgroup takes several rows, so this keeps every grid below 2^31 workgroups and a row's number within 32 bits)
-    OGMM_REQUIRE(static_cast<double>(a->B) * a->H * a->Nq < 2147483648.0 && static_cast<double>(a->B) * a->Hkv * a->Nk < 2147483648.0, "%s: more than 2^31 rows", who);
+    // (a workgroup takes 32 rows of a key head at least and up to 512 threads; a grid holds less than 2^32 threads, and rows are counted in 32 bits)
+    const int64_t G = a->H / a->Hkv, heads = static_cast<int64_t>(a->B) * a->Hkv, most = int64_t(1) << 23, blocks = std::max((a->Nq * G + 63) / 64, (int64_t(a->Nk) + 127) / 128);
+    OGMM_REQUIRE(blocks <= most && heads <= most && heads * blocks <= most, "%s: B = %d, Nq = %d, Nk = %d, H = %d, Hkv = %d are more than 2^23 blocks of 64 query rows or 128 keys of a key head",
+                 who, a->B, a->Nq, a->Nk, a->H, a->Hkv);
     const bool rows = a->B && a->Nq, keys = a->B && a->Nk;
     OGMM_REQUIRE(!rows || (a->q && a->o), "%s: missing argument", who);
     OGMM_REQUIRE(!keys || (a->k && a->v), "%s: missing argument", who);
@@ -984,7 +986,7 @@ extern "C" int ogmm_xattn_fwd(const ogmm_xattn* x, void* stream) {
     if (check("ogmm_xattn_fwd", x)) return 1;
     if (!x->B || !x->Nq) return 0;
     const Args a = forward_args(x, static_cast<float*>(x->workspace));
-    OGMM_REQUIRE(a.splits == 1 || a.workspace, "ogmm_xattn_fwd: missing workspace");
+    OGMM_REQUIRE(a.splits == 1 || (a.workspace && aligned16(a.workspace)), "ogmm_xattn_fwd: missing workspace");
     const int rows = tile_rows(x);
     return with_type(x->type, [&](auto t) {
         return with_width(x->d, [&](auto w) {

@@ -1256,7 +1256,7 @@ class _Xattn:
                 key_mask = key_mask.contiguous()
         self.held = kv_lens, q_lens, key_mask          # (alive until the kernels are enqueued)
         self.dims = B, Nq, Nk, H, Hkv, d, code
-        self.scale = d ** -0.5 if scale is None else float(scale)
+        self.scale = max(d, 1) ** -0.5 if scale is None else float(scale)
 
     def call(self, name, backward, o, rest, lse, dout=(None, 0, 0, 0), grads=(None, None, None)):
         (q, *qs), (k, *ks), (v, *vs), (g, *gs) = self.q, self.k, self.v, dout
@@ -1384,6 +1384,8 @@ def rms_norm_bwd(dy, h, weight, rstd, dh=None):
 
 def _dense(t):
     """True where a tensor's elements fill one stretch of memory without gaps or overlaps, in any order of its axes"""
+    if not t.numel():
+        return True
     n = 1
     for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s != 1), key=lambda p: p[1]):
         if stride != n:

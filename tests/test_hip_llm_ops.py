@@ -727,7 +727,7 @@ def test_refusals():
         lambda: ops.cross_attention(q, k.cpu(), v), lambda: ops.cross_attention(torch.cat([q] * 3, 3), torch.cat([k] * 3, 3), torch.cat([v] * 3, 3)),
         lambda: ops.cross_attention_bwd(q, k, v, o, lse, do[:, :4]), lambda: ops.cross_attention_bwd(q, k, v, o, lse, do.float()),
         lambda: ops.cross_attention_bwd(q, k, v, o.float(), lse, do), lambda: ops.cross_attention_bwd(q, k, v, o, lse[:, :1], do),
-        lambda: train_ops.cross_attention(q, k, v[:, :5])]
+        lambda: train_ops.cross_attention(q, k, v[:, :5]), lambda: ops.cross_attention(q[..., :0], k[..., :0], v[..., :0])]
     x, w = randn(gen(1), 6, 40, dtype=torch.bfloat16), torch.ones(40, device="cuda")
     y, h, rstd = ops.rms_norm(x, w)
     bad += [

@@ -32,7 +32,8 @@ def xattn(**kw):
 
 BAD_ATTENTION = [dict(B=-1), dict(Nq=-1), dict(Nk=-5), dict(H=0), dict(Hkv=0), dict(H=3), dict(d=0), dict(d=4), dict(d=60), dict(d=136), dict(type=3), dict(type=-1),
                  dict(q_n=255), dict(k_h=65), dict(v_b=4), dict(q=4098), dict(k=4104), dict(v=4097), dict(o=4104), dict(q=None), dict(k=None), dict(v=None), dict(o=None),
-                 dict(k_n=1 << 24), dict(q_h=1 << 24), dict(q_n=-256), dict(scale=math.nan), dict(scale=math.inf), dict(B=1 << 20, H=1 << 16, Hkv=1, Nq=1 << 20)]
+                 dict(k_n=1 << 24), dict(q_h=1 << 24), dict(q_n=-256), dict(scale=math.nan), dict(scale=math.inf), dict(B=1 << 20, H=1 << 16, Hkv=1, Nq=1 << 20),
+                 dict(B=1 << 24, H=1, Hkv=1, Nq=1, Nk=1, d=8), dict(B=1, H=1, Hkv=1, Nq=1, Nk=(1 << 30) + 1), dict(B=1 << 30, H=1 << 30, Hkv=1 << 30)]
 
 
 @pytest.mark.parametrize("kw", BAD_ATTENTION, ids=str)
@@ -124,6 +125,22 @@ def test_tensors_on_the_cpu_are_refused():
               lambda: ops.rms_norm_q8(x, w), lambda: ops.rms_norm_bwd(x, x, w, torch.ones(3)), lambda: ops.grad_norm([x]), lambda: ops.clip_grads_([x], 1.0), lambda: ops.grad_norm([None])):
         with pytest.raises(OgmmError):
             f()
+
+
+def test_a_workspace_that_is_not_aligned_is_refused(lib):
+    a = xattn(B=1, Nq=1, Nk=4096)          # few rows, many keys: cut into parts
+    assert lib.ogmm_xattn_workspace_bytes(ctypes.byref(a), 0) > 0
+    for ws in (None, 4104):
+        a.workspace = ws
+        assert lib.ogmm_xattn_fwd(ctypes.byref(a), None) != 0 and lib.ogmm_xattn_bwd(ctypes.byref(a), None) != 0
+
+
+def test_which_tensors_are_without_gaps():
+    x = torch.zeros(4, 6, 5)
+    for t in (x, x.permute(2, 0, 1), x[1:], x[:, :, :0], x[:0], torch.zeros(3, 0), torch.zeros(0, 3), torch.zeros(()), x[:, :1, :1][:1], torch.zeros(2, 3, 4, 5).contiguous(memory_format=torch.channels_last)):
+        assert ops._dense(t), (t.shape, t.stride())
+    for t in (x[:, 1:], x[:, :, ::2], torch.zeros(1, 5).expand(4, 5), x.as_strided((4, 4), (1, 1))):
+        assert not ops._dense(t), (t.shape, t.stride())
 
 
 def test_trainer_refuses_a_negative_limit():
