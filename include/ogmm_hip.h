@@ -539,7 +539,8 @@ enum { OGMM_F32 = 0, OGMM_BF16 = 1, OGMM_F16 = 2 };
  * q, k, v, dout: element strides *_b (batch), *_n (row), *_h (head), channels contiguous; addresses and strides multiples of 16 bytes.  o, dq [B][Nq][H][d] and
  * dk, dv [B][Nk][Hkv][d] contiguous, lse fp32 [B][H][Nq] (NULL in the forward: not wanted).  Every element of the outputs is written.  No atomics: repeated calls agree
  * bit for bit.  rest (16-bit types; NULL: not wanted, fp32: not used): what rounding left of o, in the type again, contiguous like o; with it the backward's sum dO o has no rounding of o
- * in it, which matters where a row looks at few keys.  workspace: ogmm_xattn_workspace_bytes(a, backward) bytes (0: NULL will do); it is used by this call alone. */
+ * in it, which matters where a row looks at few keys.  workspace: ogmm_xattn_workspace_bytes(a, backward) bytes (0: NULL will do; the fp32 backward: up to 1 GB for dS), at an address that is a
+ * multiple of 16; it is used by this call alone. */
 typedef struct ogmm_xattn {
     const void *q, *k, *v;
     int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;

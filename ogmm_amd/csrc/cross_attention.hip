@@ -483,12 +483,17 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a, int tile_
 
 // ---- backward.  Two kernels form the scores again from lse: one owns query rows and sums dQ over the keys (S^T, dP^T, dQ^T: three products), one owns keys and sums dK, dV over
 // the query rows of its G heads (S, dP, dV^T, dK^T: four products); no sum crosses workgroups but where few tiles are cut into parts, which are added in their order.
+// fp32: its matrix instructions take eight times as long for the same product, so dS is kept by the kernel that owns keys (up to 1 GB of it) and dQ is one product of it: 16 x 1024 rows
+// to 717 keys, 4 heads of 128: dq 300 -> 111 us, dk dv 480 -> 523; 1024 keys, heads of 64: 238 -> 105, 341 -> 379; of 32: 126 -> 67, 163 -> 188.  In 16 bits writing and reading dS would
+// take longer than forming it.
 struct BwdArgs : Args {
     int row_tiles, row_splits, key_tiles, key_splits;          // dq: tiles of 128 rows, parts of the keys; dk, dv: tiles of 128 keys, parts of the rows
     int delta_blocks;                                          // blocks of 64 rows to a key head
     float *lse2, *delta;                                       // [B Hkv][rows]: lse log2(e) (+inf: the row has no weights), sum of dO O
     float* top;                                                // [B Hkv][delta_blocks]: the largest |dO| (16-bit floats with five exponent bits)
     float *part_q, *part_k, *part_v;                           // parts in the outputs' own order
+    float* ds;                                                 // [B Hkv][key_tiles 128][ds_step] dS as dk, dv's kernel formed it, or null: dq forms it again
+    int64_t ds_step;                                           // (rows, up to whole tiles)
 };
 
 __device__ __forceinline__ int64_t row_offset(const Args& a, int r, int b, int hk, int64_t sb, int64_t sn, int64_t sh) {
@@ -766,6 +771,13 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
             M::mul_t(dv, lds_g, 32 * j, y);
             as_operand<T>(y, dp);
             M::mul_t(dk, lds_q, 32 * j, y);
+            if constexpr (sizeof(T) == 4)
+                if (a.ds) {          // (0 for a key that is not admitted; rows behind q_lens have 0 as it is)
+                    float* to = a.ds + (static_cast<int64_t>(bh) * a.key_tiles * 128 + key) * a.ds_step + t * QT + 32 * j + 4 * (lane >> 5);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<float4*>(to + 2 * i) = key_there ? make_float4(dp[i], dp[i + 1], dp[i + 2], dp[i + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
         }
         if (t + 1 < end) {
             put(lds + (OTHER - buffer), t + 1);
@@ -786,6 +798,77 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
         store_column<T, M>(static_cast<T*>(a.dk) + at, nullptr, dk, a.scale / up, a.d);
         store_column<T, M>(static_cast<T*>(a.dv) + at, nullptr, dv, 1.0f, a.d);
     }
+}
+
+// dQ^T = scale K^T dS^T with the dS that dk, dv's kernel left: a lane reads its row's values of 32 keys, which is the layout of a product's result
+template <int DP>
+__global__ __launch_bounds__(256, 2) void xattn_dq_of_ds_kernel(const BwdArgs a) {
+    using M = Tile<float, DP>;
+    constexpr int KT = 32;
+    using St = Stage<float, DP, KT, 256>;
+    __shared__ __attribute__((aligned(16))) char lds[2 * KT * M::PITCH];
+    uint32_t buffer = 0;
+    constexpr uint32_t OTHER = KT * M::PITCH;
+    const uint32_t item = item_of(a);
+    if (item >= a.items) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int split = item % a.row_splits, tile = item / a.row_splits % a.row_tiles, of = item / a.row_splits / a.row_tiles, hk = of % a.Hkv, b = batch_of(a, of / a.Hkv), bh = b * a.Hkv + hk;
+    const int len = clamp_len(a.kv_lens, b, a.Nk), q_rows = clamp_len(a.q_lens, b, a.Nq) * a.G;
+    const char* k = reinterpret_cast<const char*>(static_cast<const float*>(a.k) + b * a.k_b + hk * a.k_h);
+    const int64_t k_step = a.k_n * static_cast<int64_t>(sizeof(float));
+    const uint32_t chunk_off = St::chunk_offset(a.d);
+    const int row = tile * 128 + wave * 32 + (lane & 31);
+    const int tiles = tile * 128 < q_rows ? (len + KT - 1) / KT : 0, per = (tiles + a.row_splits - 1) / a.row_splits, end = min(tiles, (split + 1) * per);
+    // (a lane behind the last row reads that row's: its column of the result is its own, and becomes zeros)
+    const float* ds = a.ds + (static_cast<int64_t>(bh) * a.key_tiles * 128 + 4 * (lane >> 5)) * a.ds_step + max(0, min(row, q_rows - 1));
+    f32x16 dq[M::DB] = {};
+    u32x4 rk[St::PASSES];
+    float next[16];
+    uint8_t byte;
+    auto fetch = [&](int t) {
+        St::fetch(rk, k, k_step, t * KT, a.Nk, chunk_off);
+        byte = mask_byte(a, b, t * KT, min(len, (t + 1) * KT));
+        const float* p = ds + t * KT * a.ds_step;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[i] = p[(8 * (i / 4) + i % 4) * a.ds_step];
+    };
+    bool any = true;
+    auto put = [&](char* to, int t) {
+        const uint64_t bits[1] = {key_bits(a, byte, t * KT, min(len, (t + 1) * KT))};
+        any = bits[0] != 0;
+        St::put(to, rk, bits, bits[0] == 0xffffffffull, a.d);
+    };
+    u32x4 y[4];
+    auto take = [&] {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i / 4][i % 4] = __float_as_uint(next[i]);
+    };
+    int t = split * per;
+    if (t < end) {
+        fetch(t);
+        put(lds, t);
+        take();
+        __syncthreads();
+    }
+    for (; t < end; ++t) {
+        const bool some = __builtin_amdgcn_readfirstlane(any);          // (see the forward; without an admitted key dS may not have been written)
+        if (t + 1 < end) fetch(t + 1);
+        if (some) M::mul_t(dq, lds + buffer, 0, y);
+        if (t + 1 < end) {
+            put(lds + (OTHER - buffer), t + 1);
+            take();
+            __syncthreads();
+        }
+        buffer = OTHER - buffer;
+    }
+    if (row >= a.rows) return;
+    if (row >= q_rows)
+#pragma unroll
+        for (int db = 0; db < M::DB; ++db) dq[db] = f32x16{};
+    const int n = row / a.G, g = row - n * a.G;
+    const int64_t at = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
+    if (a.row_splits > 1) store_part<M>(a.part_q + split * (static_cast<int64_t>(a.B) * a.Nq * a.H * a.d) + at, dq, a.scale, a.d);
+    else store_column<float, M>(static_cast<float*>(a.dq) + at, nullptr, dq, a.scale, a.d);
 }
 
 // out = the parts' sum, in their order (n: a multiple of 8 values)
@@ -911,6 +994,13 @@ BwdArgs backward_args(const ogmm_xattn* x, float* ws, int64_t* floats) {
         a.part_k = take(a.key_splits * (heads * a.Nk * a.d));
         a.part_v = take(a.key_splits * (heads * a.Nk * a.d));
     }
+    a.ds_step = (a.rows + 63) / 64 * 64;
+    const int64_t scores = heads * a.key_tiles * 128 * a.ds_step;
+    if (a.type == OGMM_F32 && a.Nq && a.Nk && scores <= int64_t(1) << 28) {
+        const int64_t at = n;
+        n += scores;
+        a.ds = ws ? ws + at : reinterpret_cast<float*>(16);          // (for the sizes alone: not null)
+    }
     *floats = n;
     return a;
 }
@@ -924,12 +1014,7 @@ int launch_bwd(BwdArgs a, hipStream_t stream) {
     auto add = [&](const float* part, int parts, int64_t n, void* out) {
         xattn_add_kernel<T><<<static_cast<uint32_t>((n / 4 + 255) / 256), 256, 0, stream>>>(part, parts, n, static_cast<T*>(out));
     };
-    if (a.Nq) {
-        xattn_delta_kernel<T><<<static_cast<uint32_t>(heads * a.delta_blocks), 256, 0, stream>>>(a);
-        const uint32_t grid = deal(a, heads * a.row_tiles * a.row_splits, static_cast<int64_t>(a.row_tiles) * a.row_splits);
-        xattn_dq_kernel<T, DP><<<grid, 256, S::LDS, stream>>>(a);
-        if (a.row_splits > 1) add(a.part_q, a.row_splits, heads * a.rows * a.d, a.dq);
-    }
+    if (a.Nq) xattn_delta_kernel<T><<<static_cast<uint32_t>(heads * a.delta_blocks), 256, 0, stream>>>(a);
     if (a.Nk) {
         const uint32_t grid = deal(a, heads * a.key_tiles * a.key_splits, static_cast<int64_t>(a.key_tiles) * a.key_splits);
         xattn_dkv_kernel<T, DP><<<grid, 256, S::LDS, stream>>>(a);
@@ -937,6 +1022,17 @@ int launch_bwd(BwdArgs a, hipStream_t stream) {
             add(a.part_k, a.key_splits, heads * a.Nk * a.d, a.dk);
             add(a.part_v, a.key_splits, heads * a.Nk * a.d, a.dv);
         }
+    }
+    if (a.Nq) {
+        const uint32_t grid = deal(a, heads * a.row_tiles * a.row_splits, static_cast<int64_t>(a.row_tiles) * a.row_splits);
+        bool done = false;
+        if constexpr (sizeof(T) == 4)
+            if (a.ds) {
+                xattn_dq_of_ds_kernel<DP><<<grid, 256, 0, stream>>>(a);
+                done = true;
+            }
+        if (!done) xattn_dq_kernel<T, DP><<<grid, 256, S::LDS, stream>>>(a);
+        if (a.row_splits > 1) add(a.part_q, a.row_splits, heads * a.rows * a.d, a.dq);
     }
     return check_launch("ogmm_xattn_bwd");
 }

@@ -245,6 +245,14 @@ def test_attention_nothing():
         assert bool((lse == -math.inf).all())
 
 
+def test_attention_gradient_with_more_scores_than_are_kept():
+    """fp32 keeps dS between its two kernels up to 2^28 scores; these are more, and the second kernel forms them again"""
+    q, k, v, do = attention_case(1, 8200, 16400, 2, 2, 8, torch.float32, 11)
+    mask = torch.rand(1, 16400, generator=gen(12), device="cuda") < 0.7
+    lens = torch.tensor([16333], dtype=torch.int32, device="cuda"), torch.tensor([8190], dtype=torch.int32, device="cuda")
+    check_attention(q, k, v, do, kv_lens=lens[0], q_lens=lens[1], key_mask=mask)
+
+
 def test_attention_offsets_past_31_bits():
     """a cache of more than 2^31 bytes' and 2^31 elements' worth of keys: the last batch entry's rows are read where they are"""
     B, Nk, Hkv, d = 17, 16384 * 8, 8, 128          # 17 x 134 217 728 elements, 4.6 GB each for k and v
