@@ -1402,7 +1402,9 @@ def _grad_list(grads, name="gradient"):
     dev = _dev("%s 0" % name, grads[0])
     T = torch.Tensor
     try:          # a hundred tensors and more at a call: checked and listed all at once, and one by one only to say which is wrong
-        types = array.array("i", map(_TYPE.__getitem__, map(_DTYPE_OF, grads)))
+        dtypes = list(map(_DTYPE_OF, grads))          # (most lists are of one type: counting it takes a third of looking each up)
+        one = dtypes.count(dtypes[0]) == len(dtypes)
+        types = array.array("i", (_TYPE[dtypes[0]],)) * len(dtypes) if one else array.array("i", map(_TYPE.__getitem__, dtypes))
         ptrs, numel = array.array("Q", map(T.data_ptr, grads)), array.array("q", map(T.numel, grads))
         good = set(map(T.get_device, grads)) == {dev.index} and all(map(T.is_contiguous, grads))
     except (KeyError, TypeError, AttributeError, RuntimeError):
