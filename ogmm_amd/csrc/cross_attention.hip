@@ -1,9 +1,14 @@
 // Cross attention to states of another length (include/ogmm_hip.h, L1), forward and backward.
 //
-// Forward, one pass over the keys with a running maximum and sum.  A workgroup has four waves; a wave owns 32 query rows and forms S^T = K Q^T, so that a lane holds one
-// query's scores (32x32 result: column = lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4): maximum, exponential and sum stay inside the lane but for one exchange with
+// Forward, one pass over the keys with a running maximum and sum.  A workgroup has four waves or eight; a wave owns 32 query rows and forms S^T = K Q^T, so that a lane holds
+// one query's scores (32x32 result: column = lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4): maximum, exponential and sum stay inside the lane but for one exchange with
 // lane ^ 32, and P^T is the next product's operand as it lies, O^T = V^T P^T, with V's keys taken in the order in which the lanes hold them.  The G query heads of a key
 // head are rows of one tile (row = n G + g): their keys are read once.
+//
+// What bounds it, measured: many rows in 16 bits: matrix and vector instructions together (heads of 128: the matrix pipes are busy a third of the time, the exponentials, sums and
+// roundings take as long, and both wait at a tile's barrier): 64 x 1024 rows to 717 keys, 4 heads of 128, fp16 153 us = 630 TFLOP/s; 4 x 4096 to 4096, 16 heads over 4, bf16 724 us = 760;
+// 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16 176 us.  fp32: the fp32 matrix pipes, busy four fifths of the time (120 TFLOP/s of the 154 that a large product reaches).
+// One row: the keys' bytes: 16 requests of up to 12288 states, 8 key heads of 128, 56 us and 5 to join the parts, 302 MB at 5.4 TB/s; one token to 1024 states: 9 + 3 us, two launches' latency.
 #include "ogmm_common.h"
 #include <algorithm>
 #include <math.h>
@@ -449,7 +454,7 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
     }
 }
 
-// Joins the parts of the keys: one wave to a query row
+// Joins the parts of the keys: one wave to a query row, the loads of four parts on their way at once (512 rows of 16 parts: 4.8 us, waiting for each part's maximum first 8.4)
 template <class T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a, int tile_rows) {
     const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -501,7 +506,7 @@ __device__ __forceinline__ int64_t row_offset(const Args& a, int r, int b, int h
     return b * sb + n * sn + (hk * a.G + g) * sh;
 }
 
-// four threads to a row
+// four threads to a row, each with every fourth sixteen bytes of it (HBM-bound: 16 x 1024 x 4 fp32 rows of 128, 67 MB in 13.4 us = 5.0 TB/s)
 template <class T>
 __global__ __launch_bounds__(256) void xattn_delta_kernel(const BwdArgs a) {
     __shared__ float tops[4];
@@ -564,6 +569,7 @@ struct Bwd {
     static constexpr int TILE_BYTES = 2 * KT * M::PITCH + 2 * KT * 4, LDS = 2 * TILE_BYTES;
 };
 
+// 4 x 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16: 216 us, the matrix pipes busy 44 % of it beside the exponentials; the scores' bytes are LDS reads of K and V
 template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 128 ? 2 : 3)) void xattn_dq_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
@@ -666,6 +672,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 1
     else store_column<T, M>(static_cast<T*>(a.dq) + at, nullptr, dq, f, a.d);
 }
 
+// The same case: 305 us, matrix pipes busy half of it (two waves to a SIMD hold K, V and both sums in registers); fp32, 16 x 1024 rows to 717 keys, heads of 128: 523 us, busy three quarters
 template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
@@ -915,7 +922,8 @@ int parts_for(int64_t tiles, int64_t n, int64_t slots, int64_t least_rows = 256)
 }
 
 // Rows of a workgroup's tile.  Up to 32 rows of a key head (single tokens): one tile, whose four waves take different keys.  Eight waves share a tile's keys, which halves what each
-// does to bring them to LDS, where there are rows enough to fill the CUs with them.
+// does to bring them to LDS, where there are rows enough to fill the CUs with them and heads so narrow that two such workgroups share a CU (bf16, heads of 64: 196 us with four waves,
+// 172 with eight; fp16, heads of 128: 155 and 162).
 int tile_rows(const ogmm_xattn* a) {
     const int64_t rows = static_cast<int64_t>(a->Nq) * (a->H / a->Hkv);
     const bool narrow = a->d * (a->type == OGMM_F32 ? 2 : 1) <= 64;

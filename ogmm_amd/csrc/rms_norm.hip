@@ -8,6 +8,9 @@
 // eight loads of sixteen bytes, all in flight before the first is used) and the sum is one exchange inside a wave, or one through LDS.  The weights of a lane's
 // columns are read once and stay in registers for all the rows that its workgroup takes.  Rows may start anywhere (odd widths, strides): the part reads sixteen
 // bytes from any address; only a row's last, partial piece goes value by value.
+//
+// Measured (a large copy: 5.2 TB/s): 131072 rows of 512, fp32, with residual: 185 us = 5.8 TB/s, backward 206 us = 5.2; 8192 rows of 8192, bf16: 111 us = 4.8, backward 115 us = 4.7 and
+// 5 us for dw; 8192 rows of 4096, bf16 to 8 bits with residual: 39 us = 6.0; 5000 rows of 717, fp16, a scale to 128 columns: 9.7 us; one row: 4 us, a launch's latency.
 #include "ogmm_common.h"
 #include <algorithm>
 #include <type_traits>
@@ -325,7 +328,8 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restri
     }
 }
 
-// Lanes to a row and loads of sixteen bytes to a lane: the fewest lanes that keep a lane at four loads (narrow rows: two), so that narrow rows share a workgroup
+// Lanes to a row and loads of sixteen bytes to a lane: the fewest lanes that keep a lane at four loads (narrow rows: two), so that narrow rows share a workgroup and the sum over a
+// row takes few exchanges; the widest fp32 rows take eight
 template <class T, class F>
 int with_shape(int D, int least_lanes, F&& f) {
     constexpr int VEC = 16 / sizeof(T);
@@ -363,6 +367,7 @@ int launch_norm(const NormArgs& a, bool q8, hipStream_t stream) {
 }
 
 // dw's shares are written and read again (blocks x D x 4 bytes): two workgroups to a CU for wide rows, four for narrow ones, whose waves have fewer bytes on their way each
+// (131072 fp32 rows of 512: 206 us with two, 216 with four)
 constexpr int BWD_BLOCKS = 1024;
 
 template <class T, class W>

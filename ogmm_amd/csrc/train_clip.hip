@@ -4,6 +4,9 @@
 // kernel arguments (no copy, nothing kept between calls, capturable); each workgroup takes an equal run of their values, so a hundred small tensors
 // fill the part as well as one large one.  Squares are summed in fp64: four or eight of them in fp32 first, where
 // that is inside its range.  Every sum has a fixed order: results repeat bit for bit.
+//
+// Measured: 150 fp32 tensors, 13 M values: 14 us for the norm and 4 for finding that nothing changes (52 MB, out of the last-level cache), under 30 us of listing them on the host;
+// 400 bf16 tensors, 300 M values, clipped to fp32: 2 x 80 us for the norm = 3.8 TB/s (a large sum reads at 3.95), 3 x 128 us for the product = 4.7 TB/s (a copy: 5.2).
 #include "ogmm_common.h"
 #include <algorithm>
 #include <exception>
@@ -72,7 +75,7 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 template <int BYTES> struct __attribute__((packed, aligned(2))) Packed { uint32_t w[BYTES / 4]; };
 
 // f(values, where) over a run's values, VEC to a thread at once and AHEAD loads in flight; f1(place) for single ones: those in front of the first place at which `by` (the run's first
-// value as it is read or written) is aligned to VEC values of its own, and the last few.  A tensor may start anywhere in a bucket, and loads that straddle lines take half as long again.
+// value as it is read or written) is aligned to VEC values of its own, and the last few.  A tensor may start anywhere in a bucket, and loads that straddle lines cost more.
 template <int BYTES, int VEC, int AHEAD, class P, class F, class F1>
 __device__ __forceinline__ void over_values(const char* __restrict__ p, const P* by, uint32_t len, F&& f, F1&& f1) {
     constexpr uint32_t ROUND = THREADS * VEC;
@@ -86,7 +89,15 @@ __device__ __forceinline__ void over_values(const char* __restrict__ p, const P*
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) f(b[u], at + u * ROUND);
     }
-    for (; at + VEC <= len; at += ROUND) f(*reinterpret_cast<const Packed<BYTES>*>(p + static_cast<size_t>(at) * E), at);
+    if (at + VEC <= len) {          // what is left, fewer than AHEAD: together too
+        Packed<BYTES> b[AHEAD - 1];
+#pragma unroll
+        for (int u = 0; u < AHEAD - 1; ++u)
+            if (at + u * ROUND + VEC <= len) b[u] = *reinterpret_cast<const Packed<BYTES>*>(p + static_cast<size_t>(at + u * ROUND) * E);
+#pragma unroll
+        for (int u = 0; u < AHEAD - 1; ++u)
+            if (at + u * ROUND + VEC <= len) f(b[u], at + u * ROUND);
+    }
     if (threadIdx.x < lead) f1(threadIdx.x);
     if (threadIdx.x < tail) f1(len - tail + threadIdx.x);
 }
@@ -263,7 +274,7 @@ int fill(T& t, const std::vector<Item>& items, size_t from) {
     return n;
 }
 
-// How `chunks` are dealt: equal runs, one to a workgroup as long as that is 16 chunks or less.  (13 M values of 150 tensors: one run each 13.7 us, single chunks in turn 19; 300 M: runs
+// How `chunks` are dealt: equal runs, one to a workgroup as long as that is 16 chunks or less.  (13 M values of 150 tensors: one run each 14 us, single chunks in turn 19; 300 M: runs
 // of 65536 values keep the workgroups' reads closer together than one run each would)
 struct Deal { int blocks; uint32_t run; };
 Deal deal(uint32_t chunks) {
