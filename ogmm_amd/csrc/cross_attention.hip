@@ -8,7 +8,7 @@
 // What bounds it, measured: many rows in 16 bits: matrix and vector instructions together (heads of 128: the matrix pipes are busy a third of the time, the exponentials, sums and
 // roundings take as long, and both wait at a tile's barrier): 64 x 1024 rows to 717 keys, 4 heads of 128, fp16 153 us = 630 TFLOP/s; 4 x 4096 to 4096, 16 heads over 4, bf16 724 us = 760;
 // 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16 176 us.  fp32: the fp32 matrix pipes, busy four fifths of the time (120 TFLOP/s of the 154 that a large product reaches).
-// One row: the keys' bytes: 16 requests of up to 12288 states, 8 key heads of 128, 56 us and 5 to join the parts, 302 MB at 5.4 TB/s; one token to 1024 states: 9 + 3 us, two launches' latency.
+// One row: the keys' bytes: 16 requests of up to 12288 states, 4 key heads of 128, 56 us and 5 to join the parts, 302 MB at 5.4 TB/s; one token to 1024 states: 9 + 3 us, two launches' latency.
 #include "ogmm_common.h"
 #include <algorithm>
 #include <math.h>
