@@ -566,14 +566,14 @@ int ogmm_xattn_bwd(const ogmm_xattn* a, void* stream);
  * _q8: y in 8 bits (e4m3, OCP) instead: scales s = max|y| / 448 over the row (group = 0; [rows]) or over each `group` = 32, 64, 128 columns ([rows][ceil(D / group)]), q = e4m3(y / s);
  * s = q = 0 where max|y| / 448 is below 2^-126.
  * _bwd: g = dy w, xh = h rstd: dx = rstd (g - xh mean(g xh)) + dh (dh = the stored sum's own gradient, NULL: none; dx is the residual's gradient too), dweight = sum over the rows
- * of dy xh (weight's type); workspace: ogmm_rms_norm_bwd_workspace_bytes. */
+ * of dy xh (weight's type).  h: the stored sum (residual = NULL), or in the 16-bit types x and the residual, whose sum is then formed without the stored one's rounding; workspace: ogmm_rms_norm_bwd_workspace_bytes. */
 int ogmm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int64_t rows, int D, int type, int weight_type, float eps,
                   void* y, void* h, float* rstd, void* stream);
 int ogmm_rms_norm_q8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int64_t rows, int D, int type, int weight_type, float eps,
                      int group, void* q, float* scales, void* h, void* stream);
 int64_t ogmm_rms_norm_bwd_workspace_bytes(int64_t rows, int D);
-int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight, const float* rstd, const void* dh, int64_t lddh, int64_t rows,
-                      int D, int type, int weight_type, void* dx, void* dweight, void* workspace, void* stream);
+int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* residual, int64_t ldr, const void* weight, const float* rstd, const void* dh,
+                      int64_t lddh, int64_t rows, int D, int type, int weight_type, void* dx, void* dweight, void* workspace, void* stream);
 
 /* ---- L3: global norm of n gradient tensors and their clipping: norm = inv_scale sqrt(sum of all squares), c = min(1, max_norm / (norm + 1e-6)), and every gradient times
  * inv_scale c: in place (out = NULL) or into the fp32 tensors out[i].  grads, numel, types, out: HOST arrays of n entries (device pointers, element counts, type codes; read before the

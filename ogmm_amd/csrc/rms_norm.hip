@@ -9,7 +9,7 @@
 // columns are read once and stay in registers for all the rows that its workgroup takes.  Rows may start anywhere (odd widths, strides): the part reads sixteen
 // bytes from any address; only a row's last, partial piece goes value by value.
 //
-// Measured (a large copy: 5.2 TB/s): 131072 rows of 512, fp32, with residual: 185 us = 5.8 TB/s, backward 206 us = 5.2; 8192 rows of 8192, bf16: 111 us = 4.8, backward 115 us = 4.7 and
+// Measured (a large copy: 5.2 TB/s): 131072 rows of 512, fp32, with residual: 185 us = 5.8 TB/s, backward 206 us = 5.2; 8192 rows of 8192, bf16: 111 us = 4.8, backward 142 us = 4.7 and
 // 5 us for dw; 8192 rows of 4096, bf16 to 8 bits with residual: 39 us = 6.0; 5000 rows of 717, fp16, a scale to 128 columns: 9.7 us; one row: 4 us, a launch's latency.
 #include "ogmm_common.h"
 #include <algorithm>
@@ -201,23 +201,25 @@ __global__ __launch_bounds__(THREADS<LANES>) void rms_norm_kernel(const NormArgs
 }
 
 struct BwdArgs {
-    const void *dy, *h, *w, *dh;
+    const void *dy, *h, *r, *w, *dh;
     const float* rstd;
-    int64_t lddy, ldh, lddh, rows;
+    int64_t lddy, ldh, ldr, lddh, rows;
     int D;
     void* dx;
     float* part;          // [gridDim.x][D]: each workgroup's share of dw
 };
 
-template <class T, class W, int LANES, int ITEMS>
+// RES: the sum is formed again from its two 16-bit summands.  Its stored form is off by half a step of the type, which dw -- a sum of terms of either sign -- passes on as it is: its error
+// was 1.4 times that of its own rounding (8192 rows of 8192, bf16: 142 us, 115 from the stored sum: a fifth matrix to read, at the same 4.7 TB/s)
+template <class T, class W, int LANES, int ITEMS, bool RES>
 __global__ __launch_bounds__(THREADS<LANES>, (LANES > 256 ? 4 : 2)) void rms_norm_bwd_kernel(const BwdArgs a) {
     constexpr int VEC = 16 / sizeof(T), PER = THREADS<LANES> / LANES;
     __shared__ float lds[2 * (LANES > 64 ? LANES / 64 : 1)];
     __shared__ float share[PER > 1 ? PER * LANES * VEC : 1];
     int slot = 0;
     const int lane = threadIdx.x % LANES, D = a.D;
-    // the weights: in registers in 32 bits, or where 1024 lanes leave few of those in the rows' own 16
-    constexpr bool RAW_W = LANES > 256 && sizeof(W) == 2;
+    // the weights: in registers in 32 bits, or where 1024 lanes or four loads of every input leave few of those in the rows' own 16
+    constexpr bool RAW_W = sizeof(W) == 2 && (LANES > 256 || (RES && ITEMS > 2));
     constexpr int WVEC = 16 / sizeof(W);
     Raw w_raw[RAW_W ? ITEMS : 1];
     float w[RAW_W ? 1 : ITEMS][VEC], dw[ITEMS][VEC];
@@ -234,36 +236,43 @@ __global__ __launch_bounds__(THREADS<LANES>, (LANES > 256 ? 4 : 2)) void rms_nor
         else return w[i][k];
     };
     const float inv_d = 1.0f / D;
-    // Where the registers allow it, the next row is on its way while this one is worked on
-    constexpr bool AHEAD = LANES <= 256;
-    Raw rg[ITEMS], rh[ITEMS], ru[ITEMS];
+    // Where the registers allow it, the next row is on its way while this one is worked on (8192 rows of 8192 from the summands, four inputs of four loads: 142 us without it, 253
+    // with it, for what then spills)
+    constexpr bool AHEAD = LANES <= 256 && !(RES && ITEMS > 2);
+    Raw rg[ITEMS], rh[ITEMS], ru[ITEMS], rr[RES ? ITEMS : 1];
     float rstd = 0.0f;
-    auto fetch_row = [&](Raw (&g)[ITEMS], Raw (&h)[ITEMS], Raw (&u)[ITEMS], float& r, int64_t row) {          // (a row's lanes agree on whether it is there)
+    auto fetch_row = [&](Raw (&g)[ITEMS], Raw (&h)[ITEMS], Raw (&u)[ITEMS], Raw* x, float& r, int64_t row) {          // (a row's lanes agree on whether it is there)
         const int d = row < a.rows ? D : 0;
         r = d ? a.rstd[row] : 0.0f;
-        const T *pg = static_cast<const T*>(a.dy) + row * a.lddy, *ph = static_cast<const T*>(a.h) + row * a.ldh, *pu = static_cast<const T*>(a.dh) + row * a.lddh;
+        const T *pg = static_cast<const T*>(a.dy) + row * a.lddy, *ph = static_cast<const T*>(a.h) + row * a.ldh, *pu = static_cast<const T*>(a.dh) + row * a.lddh,
+                *pr = static_cast<const T*>(a.r) + row * a.ldr;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             g[i] = fetch<T>(pg, (i * LANES + lane) * VEC, d);
             h[i] = fetch<T>(ph, (i * LANES + lane) * VEC, d);
+            if constexpr (RES) x[i] = fetch<T>(pr, (i * LANES + lane) * VEC, d);
             if (a.dh) u[i] = fetch<T>(pu, (i * LANES + lane) * VEC, d);
         }
     };
+    auto sum = [&](int i, int k) {
+        if constexpr (RES) return value<T>(rh[i], k) + value<T>(rr[i], k);
+        else return value<T>(rh[i], k);
+    };
     const int64_t step = static_cast<int64_t>(gridDim.x) * PER;
     int64_t row = static_cast<int64_t>(blockIdx.x) * PER + threadIdx.x / LANES;
-    if constexpr (AHEAD) fetch_row(rg, rh, ru, rstd, row);
+    if constexpr (AHEAD) fetch_row(rg, rh, ru, rr, rstd, row);
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * PER; row0 < a.rows; row0 += step, row += step) {
-        if constexpr (!AHEAD) fetch_row(rg, rh, ru, rstd, row);
-        Raw ng[AHEAD ? ITEMS : 1], nh[AHEAD ? ITEMS : 1], nu[AHEAD ? ITEMS : 1];
+        if constexpr (!AHEAD) fetch_row(rg, rh, ru, rr, rstd, row);
+        Raw ng[AHEAD ? ITEMS : 1], nh[AHEAD ? ITEMS : 1], nu[AHEAD ? ITEMS : 1], nr[AHEAD && RES ? ITEMS : 1];
         float next_rstd = 0.0f;
         if constexpr (AHEAD)
-            if (row0 + step < a.rows) fetch_row(ng, nh, nu, next_rstd, row + step);
+            if (row0 + step < a.rows) fetch_row(ng, nh, nu, nr, next_rstd, row + step);
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const float g = value<T>(rg[i], k), xh = value<T>(rh[i], k) * rstd;
+                const float g = value<T>(rg[i], k), xh = sum(i, k) * rstd;
                 dw[i][k] = fmaf(g, xh, dw[i][k]);
                 dot = fmaf(g * weight(i, k), xh, dot);
             }
@@ -274,20 +283,28 @@ __global__ __launch_bounds__(THREADS<LANES>, (LANES > 256 ? 4 : 2)) void rms_nor
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(rg[i].w[j]), "+v"(rh[i].w[j]));
+                for (int j = 0; j < 4; ++j) {
+                    asm volatile("" : "+v"(rg[i].w[j]), "+v"(rh[i].w[j]));
+                    if constexpr (RES) asm volatile("" : "+v"(rr[i].w[j]));
+                }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             float dx[VEC];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                dx[k] = rstd * (value<T>(rg[i], k) * weight(i, k) - value<T>(rh[i], k) * rstd * dot);
+                dx[k] = rstd * (value<T>(rg[i], k) * weight(i, k) - sum(i, k) * rstd * dot);
                 if (a.dh) dx[k] += value<T>(ru[i], k);
             }
             store<VEC>(static_cast<T*>(a.dx) + row * D, (i * LANES + lane) * VEC, d, dx);
         }
         if constexpr (AHEAD) {
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) { rg[i] = ng[i]; rh[i] = nh[i]; ru[i] = nu[i]; }
+            for (int i = 0; i < ITEMS; ++i) {
+                rg[i] = ng[i];
+                rh[i] = nh[i];
+                ru[i] = nu[i];
+                if constexpr (RES) rr[i] = nr[i];
+            }
             rstd = next_rstd;
         }
     }
@@ -375,7 +392,10 @@ int launch_bwd(const BwdArgs& a, void* dw, hipStream_t stream) {
     return with_shape<T>(a.D, 1, [&](auto lanes, auto items) {
         constexpr int L = decltype(lanes)::value, I = decltype(items)::value;
         const int blocks = blocks_for(a.rows, THREADS<L> / L, L > 32 ? BWD_BLOCKS / 2 : BWD_BLOCKS);
-        if (blocks) rms_norm_bwd_kernel<T, W, L, I><<<blocks, THREADS<L>, 0, stream>>>(a);
+        if constexpr (sizeof(T) == 2) {
+            if (blocks && a.r) rms_norm_bwd_kernel<T, W, L, I, true><<<blocks, THREADS<L>, 0, stream>>>(a);
+        }
+        if (blocks && !a.r) rms_norm_bwd_kernel<T, W, L, I, false><<<blocks, THREADS<L>, 0, stream>>>(a);
         rms_norm_dw_kernel<W><<<(a.D + 63) / 64, 1024, 0, stream>>>(a.part, blocks, a.D, static_cast<W*>(dw));
         return check_launch("ogmm_rms_norm_bwd");
     });
@@ -425,10 +445,11 @@ extern "C" int64_t ogmm_rms_norm_bwd_workspace_bytes(int64_t rows, int D) {
     return std::max<int64_t>(1, std::min<int64_t>(rows, BWD_BLOCKS)) * D * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* weight, const float* rstd, const void* dh, int64_t lddh, int64_t rows,
+extern "C" int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* residual, int64_t ldr, const void* weight, const float* rstd, const void* dh, int64_t lddh, int64_t rows,
                                  int D, int type, int weight_type, void* dx, void* dweight, void* workspace, void* stream) {
     if (check_rows("ogmm_rms_norm_bwd", rows, D)) return 1;
     OGMM_REQUIRE(weight && dweight && workspace && (!rows || (dy && h && rstd && dx)), "ogmm_rms_norm_bwd: missing argument");
-    const BwdArgs a{dy, h, weight, dh, rstd, lddy, ldh, lddh, rows, D, dx, static_cast<float*>(workspace)};
+    OGMM_REQUIRE(!residual || type != OGMM_F32, "ogmm_rms_norm_bwd: fp32 rows are given as their sum");
+    const BwdArgs a{dy, h, residual, weight, dh, rstd, lddy, ldh, ldr, lddh, rows, D, dx, static_cast<float*>(workspace)};
     return with_types("ogmm_rms_norm_bwd", type, weight_type, [&](auto t, auto w) { return launch_bwd<decltype(t), decltype(w)>(a, dweight, as_stream(stream)); });
 }

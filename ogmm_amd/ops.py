@@ -1364,9 +1364,10 @@ def rms_norm_q8(x, weight, residual=None, eps=1e-6, group=0):
     return q, scales, h
 
 
-def rms_norm_bwd(dy, h, weight, rstd, dh=None):
-    """Backward of rms_norm(): (dx, dweight) from dy = dL/dy, the forward's h and rstd, and dh = dL/dh where the sum has readers of its own; dx is the residual's gradient too."""
-    dev, code, wcode, D, w, (h2, ldh), _ = _norm_args(h, weight, None)
+def rms_norm_bwd(dy, h, weight, rstd, dh=None, residual=None):
+    """Backward of rms_norm(): (dx, dweight) from dy = dL/dy, the forward's h and rstd, and dh = dL/dh where the sum has readers of its own; dx is the residual's gradient too.
+    In bfloat16 and float16 the forward's x and residual may stand in for h (h = x, residual = r): the sum then has no rounding in it."""
+    dev, code, wcode, D, w, (h2, ldh), (r2, ldr) = _norm_args(h, weight, residual)
     _dev("h", h, dy=dy, rstd=rstd, dh=dh)
     for n, t in (("dy", dy), ("dh", dh)):
         if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
@@ -1378,7 +1379,7 @@ def rms_norm_bwd(dy, h, weight, rstd, dh=None):
     dx = h.new_empty(h.shape)
     dw = w.new_empty(D)
     ws = torch.empty(_lib.load().ogmm_rms_norm_bwd_workspace_bytes(h2.shape[0], D), dtype=torch.uint8, device=dev)
-    _call_on(dev, "ogmm_rms_norm_bwd", dy2.data_ptr(), lddy, h2.data_ptr(), ldh, w.data_ptr(), rstd.data_ptr(), _ptr(dh2), lddh, h2.shape[0], D, code, wcode, dx.data_ptr(), dw.data_ptr(), ws.data_ptr())
+    _call_on(dev, "ogmm_rms_norm_bwd", dy2.data_ptr(), lddy, h2.data_ptr(), ldh, _ptr(r2), ldr, w.data_ptr(), rstd.data_ptr(), _ptr(dh2), lddh, h2.shape[0], D, code, wcode, dx.data_ptr(), dw.data_ptr(), ws.data_ptr())
     return dx, dw
 
 

@@ -817,12 +817,13 @@ def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=Non
 
 
 class _RmsNorm(torch.autograd.Function):
-    """ops.rms_norm with its gradient; the backward reads the stored sum and one rstd a row"""
+    """ops.rms_norm with its gradient; the backward reads one rstd a row and the stored sum, in the 16-bit types its two summands"""
 
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, h, rstd = ops.rms_norm(x, weight, residual, eps)
-        ctx.save_for_backward(h, weight, rstd)
+        apart = residual is not None and x.dtype != torch.float32
+        ctx.save_for_backward(x if apart else h, residual if apart else None, weight, rstd)
         ctx.has_residual = residual is not None
         ctx.set_materialize_grads(False)
         return (y, h) if ctx.has_residual else y
@@ -830,10 +831,10 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
+        h, residual, weight, rstd = ctx.saved_tensors
         if dy is None:          # only the sum is used further on
             return dh, None, (dh if ctx.has_residual else None), None
-        dx, dw = ops.rms_norm_bwd(dy, h, weight, rstd, dh)
+        dx, dw = ops.rms_norm_bwd(dy, h, weight, rstd, dh, residual)
         return dx, dw, (dx if ctx.has_residual else None), None
 
 

@@ -323,6 +323,29 @@ def test_norm_gradient(dtype, R, D):
         assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS.get)
+@pytest.mark.parametrize("R,D", [(1, 3), (102, 458), (50, 130), (33, 1024), (20, 5003), (12, 16384), (9, 32768)])
+def test_norm_gradient_from_the_summands(dtype, R, D):
+    """x and residual in place of their stored sum: the gradients are those of the sum itself, and so through autograd"""
+    from ogmm_amd import ops, train_ops
+    g = gen(R + D)
+    x, r, dy, dh = (randn(g, R, D, dtype=dtype) for _ in range(4))
+    w = (1 + 0.3 * randn(g, D)).to(dtype)
+    _, h, rstd = ops.rms_norm(x, w, r)
+    H, RS, _ = norm_reference(x, w, r, 1e-6)
+    G, XH = dy.double() * w.double(), H * RS
+    DX = RS * (G - XH * (G * XH).mean(dim=1, keepdim=True)) + dh.double()
+    size = RS * (G.abs() + XH.abs() * (G * XH).abs().mean(dim=1, keepdim=True)) + dh.double().abs()
+    DW = (dy.double() * XH).sum(dim=0)
+    dx, dw = ops.rms_norm_bwd(dy, x, w, rstd, dh, residual=r)
+    # as test_norm_gradient, with rstd known to NORM_U and the sum to U: 41 U for each of the three factors of xh mean(g xh)
+    close(dx, DX, (72 + 3 * 41) * U * size + half_step(dtype) * DX.abs() + tiny(dtype), "dx")
+    close(dw, DW, (min(R, 64 + R // 64) + 48 + 41) * U * (dy.double() * XH).abs().sum(dim=0) + half_step(dtype) * DW.abs() + tiny(dtype), "dw")
+    leaves = [t.clone().requires_grad_() for t in (x, r, w)]
+    grads = torch.autograd.grad(train_ops.rms_norm(leaves[0], leaves[2], leaves[1]), leaves, (dy, dh))
+    assert torch.equal(grads[0], dx) and torch.equal(grads[1], dx) and torch.equal(grads[2], dw)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 def test_norm_autograd_matches_differences(dtype):
     from ogmm_amd import train_ops
@@ -742,7 +765,8 @@ def test_refusals():
         lambda: ops.rms_norm(x, w[:39]), lambda: ops.rms_norm(x, w.half()), lambda: ops.rms_norm(x, w, x[:3]), lambda: ops.rms_norm(x, w, x.float()), lambda: ops.rms_norm(x.int(), w),
         lambda: ops.rms_norm(x, w, eps=-1.0), lambda: ops.rms_norm(x, w.cpu()), lambda: ops.rms_norm(torch.empty(1, 40000, device="cuda"), torch.empty(40000, device="cuda")),
         lambda: ops.rms_norm(x[:, :0], w[:0]), lambda: ops.rms_norm_q8(x, w, group=48), lambda: ops.rms_norm_q8(x, w, group=256), lambda: ops.rms_norm_bwd(y, h, w, rstd[:3]),
-        lambda: ops.rms_norm_bwd(y.float(), h, w, rstd), lambda: ops.rms_norm_bwd(y, h, w, rstd, y[:2]), lambda: ops.rms_norm_bwd(y, h, w, rstd.double())]
+        lambda: ops.rms_norm_bwd(y.float(), h, w, rstd), lambda: ops.rms_norm_bwd(y, h, w, rstd, y[:2]), lambda: ops.rms_norm_bwd(y, h, w, rstd.double()), lambda: ops.rms_norm_bwd(y, h, w, rstd, residual=y[:3]),
+        lambda: ops.rms_norm_bwd(y.float(), h.float(), w, rstd, residual=h.float())]
     a = torch.ones(100, device="cuda")
     bad += [
         lambda: ops.grad_norm([]), lambda: ops.clip_grads_([a, a], 1.0), lambda: ops.clip_grads_([a[:60], a[50:]], 1.0), lambda: ops.clip_grads_([a], -1.0), lambda: ops.clip_grads_([a], math.nan),

@@ -79,7 +79,7 @@ def test_norm_refuses(lib, kw):
     assert lib.ogmm_rms_norm_q8(*norm_args(**kw), 0, 4096, 4096, None, None) != 0
     a = norm_args(**kw)
     if "eps" not in kw and "x" not in kw:
-        assert lib.ogmm_rms_norm_bwd(4096, 64, 4096, 64, a[4], 4096, None, 0, a[5], a[6], a[7], a[8], 4096, 4096, 4096, None) != 0
+        assert lib.ogmm_rms_norm_bwd(4096, 64, 4096, 64, None, 0, a[4], 4096, None, 0, a[5], a[6], a[7], a[8], 4096, 4096, 4096, None) != 0
 
 
 def test_norm_refuses_missing_outputs_and_groups(lib):
@@ -89,6 +89,7 @@ def test_norm_refuses_missing_outputs_and_groups(lib):
         assert lib.ogmm_rms_norm_q8(*norm_args(), group, 4096, 4096, None, None) != 0
     assert lib.ogmm_rms_norm_q8(*norm_args(), 0, 4096, None, None, None) != 0
     assert lib.ogmm_rms_norm(*norm_args(rows=0, x=None), None, None, None, None) == 0
+    assert lib.ogmm_rms_norm_bwd(4096, 64, 4096, 64, 4096, 64, 4096, 4096, None, 0, 10, 64, 0, 0, 4096, 4096, 4096, None) != 0          # fp32 rows as two summands
     assert lib.ogmm_rms_norm_bwd_workspace_bytes(-1, 8) == -1 and lib.ogmm_rms_norm_bwd_workspace_bytes(10, 8) >= 10 * 8 * 4
 
 
