@@ -5,7 +5,7 @@ import torch as _torch
 
 # HIP graph replay (GMMReg.capture_graph, Trainer(graph=True)) on ROCm 7.2: with the runtime's "graph packet capture" path on (its default), a replayed
 # graph faults on GPU memory once a few thousand ordinary kernel launches have gone through the same device between two replays -- found with the
-# ~1800-node training step (tools/train_capture_debug.py launch30000 / twin), gone with DEBUG_CLR_GRAPH_PACKET_CAPTURE=0.  The runtime reads the flag
+# ~1800-node training step, gone with DEBUG_CLR_GRAPH_PACKET_CAPTURE=0.  The runtime reads the flag
 # when it initialises, so it is set here, at import; `graph_replay_safe()` tells whether that was early enough.
 def _runtime_untouched():
     """True if nothing in this process has initialised the HIP runtime yet.  torch.cuda.is_initialized() only tracks torch's own lazy initialisation;

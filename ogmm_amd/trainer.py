@@ -152,7 +152,7 @@ class Trainer:
         (loss * scale).backward()
         # Detached: nothing a caller keeps from one step may hold that step's autograd graph alive into the next one.  (Not only tidiness: with the
         # previous step's outputs -- and through their grad_fn its graph -- still alive, ending the capture of a recorded step crashed inside the HIP
-        # runtime on this ROCm; tools/train_capture_debug.py reproduces it.)
+        # runtime on this ROCm.)
         return (tuple(o.detach() for o in out), loss.detach(), {k: v.detach() for k, v in parts.items()}, fwd_flag,
                 ((flags if flags is not None else flag).clone() if flag is not None else None))
 
