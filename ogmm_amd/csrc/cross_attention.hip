@@ -495,7 +495,9 @@ struct BwdArgs : Args {
     int row_tiles, row_splits, key_tiles, key_splits;          // dq: tiles of 128 rows, parts of the keys; dk, dv: tiles of 128 keys, parts of the rows
     int delta_blocks;                                          // blocks of 64 rows to a key head
     float *lse2, *delta;                                       // [B Hkv][rows]: lse log2(e) (+inf: the row has no weights), sum of dO O
-    float* top;                                                // [B Hkv][delta_blocks]: the largest |dO| (16-bit floats with five exponent bits)
+    // fp16: [B Hkv][rows] |dO| of a row; [B Hkv][delta_blocks] the largest |dO| and |sum of dO O|; [B Hkv][key_tiles][4] the largest |v| of a wave's keys (2-norms)
+    float *size, *top_v;
+    float2* top;
     float *part_q, *part_k, *part_v;                           // parts in the outputs' own order
     float* ds;                                                 // [B Hkv][key_tiles 128][ds_step] dS as dk, dv's kernel formed it, or null: dq forms it again
     int64_t ds_step;                                           // (rows, up to whole tiles)
@@ -506,15 +508,19 @@ __device__ __forceinline__ int64_t row_offset(const Args& a, int r, int b, int h
     return b * sb + n * sn + (hk * a.G + g) * sh;
 }
 
+template <class T> constexpr bool NARROW = std::is_same_v<T, _Float16>;          // few exponent bits
+template <class T> constexpr float P_LOG2 = NARROW<T> ? 14.0f : 0.0f;
+template <class T> constexpr float P_POWER = NARROW<T> ? 0x1p14f : 1.0f;
+
 // four threads to a row, each with every fourth sixteen bytes of it (HBM-bound: 16 x 1024 x 4 fp32 rows of 128, 67 MB in 13.4 us = 5.0 TB/s)
 template <class T>
 __global__ __launch_bounds__(256) void xattn_delta_kernel(const BwdArgs a) {
-    __shared__ float tops[4];
+    __shared__ float2 tops[4];
     constexpr int VEC = 16 / sizeof(T);
     typedef T tv __attribute__((ext_vector_type(VEC)));
     const int block = blockIdx.x % a.delta_blocks, bh = blockIdx.x / a.delta_blocks, hk = bh % a.Hkv, b = bh / a.Hkv;
     const int r = block * 64 + (threadIdx.x >> 2);
-    float delta = 0.0f, top = 0.0f;
+    float delta = 0.0f, size = 0.0f;
     if (r < a.rows) {
         const int n = r / a.G, g = r - n * a.G;
         const float lse = a.lse[(static_cast<int64_t>(b) * a.H + hk * a.G + g) * a.Nq + n];
@@ -530,36 +536,42 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(const BwdArgs a) {
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     delta = fmaf(static_cast<float>(x[k]) + static_cast<float>(z[k]), static_cast<float>(y[k]), delta);
-                    top = fmaxf(top, fabsf(static_cast<float>(y[k])));
+                    if constexpr (NARROW<T>) size = fmaf(static_cast<float>(y[k]), static_cast<float>(y[k]), size);
                 }
             }
         }
         delta += __shfl_xor(delta, 1, 64);
         delta += __shfl_xor(delta, 2, 64);
+        if constexpr (NARROW<T>) {
+            size += __shfl_xor(size, 1, 64);
+            size += __shfl_xor(size, 2, 64);
+            size = sqrtf(size);
+        }
         if ((threadIdx.x & 3) == 0) {
-            a.lse2[static_cast<int64_t>(bh) * a.rows + r] = there ? lse * LOG2E : INFINITY;
-            a.delta[static_cast<int64_t>(bh) * a.rows + r] = delta;
+            const int64_t at = static_cast<int64_t>(bh) * a.rows + r;
+            a.lse2[at] = there ? lse * LOG2E : INFINITY;
+            a.delta[at] = delta;
+            if constexpr (NARROW<T>) a.size[at] = size;
         }
     }
-    if constexpr (std::is_same_v<T, _Float16>) {
-        top = wave_max(top);
-        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    if constexpr (NARROW<T>) {
+        size = wave_max(size);
+        const float top = wave_max(fabsf(delta));
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = make_float2(size, top);
         __syncthreads();
-        if (threadIdx.x == 0) a.top[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        if (threadIdx.x == 0)
+            a.top[blockIdx.x] = make_float2(fmaxf(fmaxf(tops[0].x, tops[1].x), fmaxf(tops[2].x, tops[3].x)), fmaxf(fmaxf(tops[0].y, tops[1].y), fmaxf(tops[2].y, tops[3].y)));
     }
 }
 
-// dS as an fp16 operand: times a power of two that brings the largest |dO| of the rows that share a key head to [1, 2), so that a gradient of any size keeps its precision
-// where fp16's exponents end (fp32 and bf16 have the range).  |P (dP - delta)| is half of max |dP| at most: nothing overflows while a key's |v| sum to 65504 or less.
-template <class T>
-__device__ __forceinline__ float gradient_scale(const BwdArgs& a, int bh) {
-    if constexpr (std::is_same_v<T, _Float16>) {
-        float top = 0.0f;
-        for (int i = threadIdx.x & 63; i < a.delta_blocks; i += 64) top = fmaxf(top, a.top[static_cast<int64_t>(bh) * a.delta_blocks + i]);
-        top = wave_max(top);
-        if (top > 0.0f && top < INFINITY) return __uint_as_float(static_cast<uint32_t>(254 - min(253, static_cast<int>(__float_as_uint(top) >> 23))) << 23);
-    }
-    return 1.0f;
+// fp16 ends at 2^-14 and at 65504, so P and dS are operands times powers of two there, which the sums are rid of at the end.  P <= 1 stands at 2^14: half a step is 2^-39 at least, and there is room for
+// scores so large that fp32 knows them to within 1.  |dS_ij| = P_ij |dO_i v_j - delta_i| is at most |dO_i| |v_j| + |delta_i| (2-norms): dQ takes that bound for each of its rows, with the longest v,
+// dK for each of its keys, with the largest |dO| and |delta|, and brings it to [2^13, 2^14].  Half a step of a small dS is 2^-38 of its bound: with 4096 keys of
+// like weights 2^-14 of the dS of a row that lies 2^10 below its head's largest, where fp16's own rounding is 2^-11.  Nothing overflows.  (A power that follows the values as they come would leave
+// 2^-21 of each sum's own largest, for 2 to 10 % of the kernels' time.)
+__device__ __forceinline__ float power_for(float bound) {
+    if (!(bound > 0.0f && bound < INFINITY)) return 1.0f;          // (no gradient at all, or NaN and infinities: so are the sums)
+    return __uint_as_float(static_cast<uint32_t>(min(254, 267 - static_cast<int>(__float_as_uint(bound) >> 23))) << 23);
 }
 
 template <class T, int DP>
@@ -591,12 +603,19 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 1
     const int row = tile * 128 + wave * 32 + (lane & 31);
     const bool row_there = row < q_rows;
     // (a negative scale turns the queries' signs, so that -inf is below every score; scale = 0: no score)
-    const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E, up = gradient_scale<T>(a, bh);
+    const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
+    float up = 1.0f;          // dS's power of two, the same in both halves of a column
     u32x4 q[M::CHUNKS], go[M::CHUNKS];
     float lse2 = INFINITY, delta = 0.0f;
     {
         const int64_t at = static_cast<int64_t>(bh) * a.rows + row;
         if (row_there) { lse2 = a.lse2[at]; delta = a.delta[at]; }
+        if constexpr (NARROW<T>) {
+            float top = 0.0f;
+            for (int i = lane; i < a.key_tiles * 4; i += 64) top = fmaxf(top, a.top_v[static_cast<int64_t>(bh) * a.key_tiles * 4 + i]);
+            top = wave_max(top);
+            if (row_there) up = power_for(fmaf(a.size[at], top, fabsf(delta)));
+        }
         const char* pq = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + row_offset(a, row, b, hk, a.q_b, a.q_n, a.q_h));
         const char* pg = reinterpret_cast<const char*>(static_cast<const T*>(a.dout) + row_offset(a, row, b, hk, a.do_b, a.do_n, a.do_h));
         const uint32_t flip = a.scale < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
@@ -692,7 +711,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
     const bool key_there = key < len && (!a.key_mask || a.key_mask[b * a.mask_b + key]);
     // (all four waves take part in the tiles of rows, or none: a tile of keys without one that is admitted)
     const bool any = (key_bits(a, mask_byte(a, b, tile * 128, len), tile * 128, len) | key_bits(a, mask_byte(a, b, tile * 128 + 64, len), tile * 128 + 64, len)) != 0;
-    const float c = a.scale * LOG2E, up = gradient_scale<T>(a, bh);
+    const float c = a.scale * LOG2E;
+    float up = 1.0f;          // dS's power of two, the same in both halves of a column
     u32x4 k[M::CHUNKS], v[M::CHUNKS];
     {
         const char* pk = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + b * a.k_b + key * a.k_n + hk * a.k_h);
@@ -706,6 +726,25 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
                 v[s] = *reinterpret_cast<const u32x4*>(pv + at);
             }
         }
+    }
+    if constexpr (NARROW<T>) {
+        float size = 0.0f, top = 0.0f, top_delta = 0.0f;
+        typedef T t8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int s = 0; s < M::CHUNKS; ++s) {
+            const t8 x = __builtin_bit_cast(t8, v[s]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) size = fmaf(static_cast<float>(x[i]), static_cast<float>(x[i]), size);
+        }
+        size = sqrtf(add_halves(size));
+        for (int i = lane; i < a.delta_blocks; i += 64) {
+            const float2 t = a.top[static_cast<int64_t>(bh) * a.delta_blocks + i];
+            top = fmaxf(top, t.x);
+            top_delta = fmaxf(top_delta, t.y);
+        }
+        up = power_for(fmaf(wave_max(top), size, wave_max(top_delta))) / P_POWER<T>;          // (its dS comes with P's power)
+        size = wave_max(size);
+        if (split == 0 && lane == 0) a.top_v[(static_cast<int64_t>(bh) * a.key_tiles + tile) * 4 + wave] = size;
     }
     const int tiles = any ? (q_rows + QT - 1) / QT : 0, per = (tiles + a.key_splits - 1) / a.key_splits, end = min(tiles, (split + 1) * per);
     f32x16 dk[M::DB] = {}, dv[M::DB] = {};
@@ -748,7 +787,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
         const uint64_t bits[1] = {left >= 64 ? ~uint64_t(0) : (uint64_t(1) << left) - 1};          // rows behind q_lens become zeros
         St::put(to, rq, bits, left >= QT, a.d);
         St::put(to + QT * M::PITCH, rg, bits, left >= QT, a.d);
-        if (threadIdx.x < 2 * QT) reinterpret_cast<float*>(to + 2 * QT * M::PITCH)[threadIdx.x] = -r_stat;
+        // (P's power comes in here: where the value is fetched, the workgroup would wait for it: 64 x 1024 rows to 717 keys, 4 heads of 128, fp16: 366 us instead of 325)
+        if (threadIdx.x < 2 * QT) reinterpret_cast<float*>(to + 2 * QT * M::PITCH)[threadIdx.x] = (threadIdx.x < QT ? P_LOG2<T> : 0.0f) - r_stat;
     };
     int t = split * per;
     if (t < end) {
@@ -798,12 +838,13 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv
     if (!key_there)
 #pragma unroll
         for (int db = 0; db < M::DB; ++db) dk[db] = dv[db] = f32x16{};
+    const float fk = a.scale / (up * P_POWER<T>), fv = 1.0f / P_POWER<T>;
     if (a.key_splits > 1) {
-        store_part<M>(a.part_k + split * all + at, dk, a.scale / up, a.d);
-        store_part<M>(a.part_v + split * all + at, dv, 1.0f, a.d);
+        store_part<M>(a.part_k + split * all + at, dk, fk, a.d);
+        store_part<M>(a.part_v + split * all + at, dv, fv, a.d);
     } else {
-        store_column<T, M>(static_cast<T*>(a.dk) + at, nullptr, dk, a.scale / up, a.d);
-        store_column<T, M>(static_cast<T*>(a.dv) + at, nullptr, dv, 1.0f, a.d);
+        store_column<T, M>(static_cast<T*>(a.dk) + at, nullptr, dk, fk, a.d);
+        store_column<T, M>(static_cast<T*>(a.dv) + at, nullptr, dv, fv, a.d);
     }
 }
 
@@ -996,7 +1037,11 @@ BwdArgs backward_args(const ogmm_xattn* x, float* ws, int64_t* floats) {
     };
     a.lse2 = take(heads * a.rows);
     a.delta = take(heads * a.rows);
-    a.top = take(heads * a.delta_blocks);
+    if (a.type == OGMM_F16) {
+        a.size = take(heads * a.rows);
+        a.top = reinterpret_cast<float2*>(take(heads * a.delta_blocks * 2));
+        a.top_v = take(heads * a.key_tiles * 4);
+    }
     if (a.row_splits > 1) a.part_q = take(a.row_splits * (heads * a.rows * a.d));
     if (a.key_splits > 1) {
         a.part_k = take(a.key_splits * (heads * a.Nk * a.d));

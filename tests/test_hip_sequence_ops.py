@@ -1,0 +1,98 @@
+"""GPU: cross attention, RMS norm and gradient clipping where values, rows or lists differ by orders of magnitude, where NaN and infinities stand, and at the sizes from which the
+kernels take other routes; against plain evaluations in 64 bits.  The bounds count roundings as in test_hip_llm_ops.py."""
+import math
+
+import pytest
+import torch
+
+import ogmm_amd          # noqa: F401  (before anything touches the GPU: it switches the runtime's graph packet capture off)
+from test_hip_llm_ops import U, attention_case, gen
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- cross attention: gradients row by row
+def heads(x):
+    return x.double().permute(0, 2, 1, 3).contiguous()          # [B, heads, n, d]
+
+
+def row_gradients(q, k, v, do):
+    """{name: (gradient in 64 bits, bound of each row's error in the 2-norm)}, as many key heads as query heads, fp16.
+
+    A row's error is a sum of roundings that know nothing of each other: it is held to four times the root of their squares' sum (each at its largest, h = 2^-11 of an operand).
+    dS and P stand as fp16 operands at h, and not below 2^-38 of the bound that dS has over its query row (dq) or key (dk), |dO| |v| + |D|, 2^-39 for P.  Before that comes fp32: a score is d
+    products (4 sqrt(d) roundings of its largest product), a row's weights have one sum over the keys in common.  The row sums D = dO o are formed from an o whose weights were rounded:
+    P_ij e_D enters dS_ij."""
+    B, Nq, H, d = q.shape
+    Nk, h, a, c = k.shape[1], 2.0 ** -11, 2.0 ** -25, d ** -0.5
+    Q, K, V, DO = map(heads, (q, k, v, do))
+
+    def T(x):
+        return x.transpose(2, 3).contiguous()
+
+    def size(x):
+        return (x * x).sum(dim=3, keepdim=True)
+
+    S = Q @ T(K) * c
+    r = U * (4 * math.sqrt(d) * float(Q.abs().max() * K.abs().max()) * c + 4 * math.sqrt(Nk) + 4 * float(S.abs().max()) + 32)
+    P = torch.softmax(S, dim=3)
+    dP = DO @ T(V)
+    D = (P * dP).sum(dim=3, keepdim=True)
+    dS = P * (dP - D)
+    e_d = 4 * (h + r) * (P * dP).square().sum(dim=3, keepdim=True).sqrt()          # [.., Nq, 1]
+    dq, dk, dv = dS @ K * c, T(dS) @ Q * c, T(P) @ DO
+    e_ds = (h + r) * dS.abs()
+    long_v, long_do = size(V).sqrt(), size(DO).sqrt()
+    low_q = 2.0 ** -38 * (long_do * long_v.amax(dim=2, keepdim=True) + D.abs())
+    low_k = 2.0 ** -38 * T(long_v * long_do.amax(dim=2, keepdim=True) + D.abs().amax(dim=2, keepdim=True))
+    e_dq = 4 * c * ((e_ds + low_q).square() @ size(K)).sqrt() + c * e_d * size(P @ K).sqrt()
+    e_dk = 4 * c * (T((e_ds + low_k).square() + (P * e_d).square()) @ size(Q)).sqrt()
+    e_dv = 4 * (T(((h + r) * P + 2.0 ** -39).square()) @ size(DO)).sqrt()
+    out = {}
+    for name, x, e in (("dq", dq, e_dq), ("dk", dk, e_dk), ("dv", dv, e_dv)):
+        out[name] = x.permute(0, 2, 1, 3), (e + (h + r) * size(x).sqrt() + a * math.sqrt(d)).permute(0, 2, 1, 3)[..., 0]
+    return out
+
+
+def check_row_gradients(q, k, v, do):
+    from ogmm_amd import ops
+    want = row_gradients(q, k, v, do)
+    o, lse, rest = ops.cross_attention(q, k, v, need_lse=True, need_rest=True)
+    for name, x in zip(("dq", "dk", "dv"), ops.cross_attention_bwd(q, k, v, o, lse, do, rest=rest)):
+        off = (x.double() - want[name][0]).square().sum(dim=3).sqrt()
+        bad = ~(off <= want[name][1])
+        assert not bad.any(), "%s: %d of %d rows beyond the bound; worst off by %.3g of its size at a bound of %.3g" % (
+            name, int(bad.sum()), bad.numel(), *(float((x / want[name][0].square().sum(dim=3).sqrt())[bad].max()) for x in (off, want[name][1])))
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("rows", ["one above the others", "half of them small", "each its own"])
+def test_attention_fp16_rows_whose_gradients_differ(rows, d):
+    """the gradient of a small row is its own, however large the others that share its key head are"""
+    Nq, Nk = 256, 4096
+    q, k, v, do = attention_case(1, Nq, Nk, 2, 1, d, torch.float16, 5 * d)
+    if rows == "one above the others":
+        by = torch.full((Nq,), 2.0 ** -6, device="cuda")
+        by[77] = 2.0 ** 4
+    elif rows == "half of them small":
+        by = torch.where(torch.arange(Nq, device="cuda") % 2 == 0, 2.0 ** 0, 2.0 ** -7)
+    else:
+        by = 2.0 ** torch.arange(Nq, device="cuda").remainder(14).sub(7).float()
+    check_row_gradients(q, k, v, (do.float() * by[None, :, None, None]).half())
+
+
+@pytest.mark.parametrize("Nq,Nk,d", [(64, 400_001, 32), (33, 65_536, 128)])
+def test_attention_fp16_gradients_of_many_keys(Nq, Nk, d):
+    """weights of 1 / Nk each, far below fp16's normal numbers"""
+    q, k, v, do = attention_case(1, Nq, Nk, 1, 1, d, torch.float16, Nk, size=0.3)
+    check_row_gradients(q, k, v, do)
+
+
+def test_attention_fp16_gradients_of_large_values():
+    """values whose magnitudes add up to more than fp16 holds: dO v and dS leave its range, the gradients do not"""
+    q, k, _, _ = attention_case(1, 50, 40, 1, 1, 128, torch.float16, 31, size=0.2)
+    g = gen(32)
+    sign = torch.where(torch.rand(128, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    v = (30000.0 * sign * torch.where(torch.arange(40, device="cuda") % 2 == 0, -1.0, 1.0)[:, None] * (0.5 + 0.5 * torch.rand(40, 128, generator=g, device="cuda"))).half()[None, :, None]
+    do = (2.0 ** -12 * sign * (0.5 + torch.rand(50, 128, generator=g, device="cuda"))).half()[None, :, None]
+    check_row_gradients(q, k, v, do)
