@@ -684,6 +684,9 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 1
         buffer = OTHER - buffer;
     }
     if (row >= a.rows) return;
+    if (!row_there)          // (behind q_lens: a NaN of its neighbours' keys has come to its zeros)
+#pragma unroll
+        for (int db = 0; db < M::DB; ++db) dq[db] = f32x16{};
     const int n = row / a.G, g = row - n * a.G;
     const int64_t at = ((static_cast<int64_t>(b) * a.Nq + n) * a.H + hk * a.G + g) * a.d;
     const float f = a.scale / up;

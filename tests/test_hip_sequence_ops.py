@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ogmm_amd          # noqa: F401  (before anything touches the GPU: it switches the runtime's graph packet capture off)
-from test_hip_llm_ops import U, attention_case, gen
+from test_hip_llm_ops import IDS, TYPES, U, attention_case, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,34 @@ def test_attention_fp16_gradients_of_large_values():
     v = (30000.0 * sign * torch.where(torch.arange(40, device="cuda") % 2 == 0, -1.0, 1.0)[:, None] * (0.5 + 0.5 * torch.rand(40, 128, generator=g, device="cuda"))).half()[None, :, None]
     do = (2.0 ** -12 * sign * (0.5 + torch.rand(50, 128, generator=g, device="cuda"))).half()[None, :, None]
     check_row_gradients(q, k, v, do)
+
+
+# ---------------------------------------------------------------------------------------------- cross attention: NaN, infinities, rows that nobody has
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("Nq,G,Nk", [(5, 1, 90), (40, 1, 90), (200, 2, 300), (3, 4, 4000)])
+def test_attention_rows_behind_their_lengths_beside_bad_keys(dtype, Nq, G, Nk):
+    """rows behind q_lens give zeros (lse: -inf) in every output also where an admitted key or value is NaN or infinite"""
+    from ogmm_amd import ops
+    B, H, d = 2, 4, 64
+    q, k, v, do = attention_case(B, Nq, Nk, H, G, d, dtype, 3)
+    q_lens = torch.tensor([Nq // 2, 0], dtype=torch.int32, device="cuda")
+    for at, what in ((k, math.nan), (v, math.nan), (v, math.inf), (k, -math.inf)):
+        kept = at[:, 3].clone()
+        at[:, 3] = what
+        o, lse, rest = ops.cross_attention(q, k, v, q_lens=q_lens, need_lse=True, need_rest=True)
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, do, q_lens=q_lens, rest=rest)
+        for b in range(B):
+            n = int(q_lens[b])
+            assert float(o[b, n:].abs().max()) == 0.0 and float(dq[b, n:].abs().max()) == 0.0 and bool((lse[b, :, n:] == -math.inf).all())
+        assert float(dk[1].abs().max()) == 0.0 and float(dv[1].abs().max()) == 0.0          # (no row at all)
+        at[:, 3] = kept
+
+
+def test_attention_rows_behind_their_lengths_beside_bad_keys_with_more_scores_than_are_kept():
+    from ogmm_amd import ops
+    q, k, v, do = attention_case(1, 8200, 16400, 2, 2, 8, torch.float32, 11)
+    q_lens = torch.tensor([8100], dtype=torch.int32, device="cuda")
+    k[0, 5] = math.nan
+    o, lse = ops.cross_attention(q, k, v, q_lens=q_lens, need_lse=True)
+    dq, _, _ = ops.cross_attention_bwd(q, k, v, o, lse, do, q_lens=q_lens)
+    assert float(dq[0, 8100:].abs().max()) == 0.0 and bool(torch.isnan(dq[0, :8100]).all())
