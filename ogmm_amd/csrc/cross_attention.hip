@@ -412,7 +412,7 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w * 32 + (lane & 31)].x);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));          // (a wave without a key: 0, also where no wave has one)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -422,8 +422,8 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
         const int out_row = tile * 32 + r;
         float2 all = make_float2(-INFINITY, 0.0f);
         for (int w = 0; w < 4; ++w) all.x = fmaxf(all.x, ml[w * 32 + r].x);
-        for (int w = 0; w < 4; ++w)
-            if (ml[w * 32 + r].x != -INFINITY) all.y += ml[w * 32 + r].y * __builtin_amdgcn_exp2f(ml[w * 32 + r].x - all.x);
+        // (a wave whose scores are all NaN has a sum that is NaN, at a maximum of -inf)
+        for (int w = 0; w < 4; ++w) all.y += ml[w * 32 + r].y * __builtin_amdgcn_exp2f(ml[w * 32 + r].x - (all.x == -INFINITY ? 0.0f : all.x));
         if (out_row < a.rows) {
             const int on = out_row / a.G, og = out_row - on * a.G;
             const float inv = a.splits > 1 ? 1.0f : all.y > 0.0f ? 1.0f / all.y : all.y;

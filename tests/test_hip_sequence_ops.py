@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ogmm_amd          # noqa: F401  (before anything touches the GPU: it switches the runtime's graph packet capture off)
-from test_hip_llm_ops import IDS, TYPES, U, attention_case, gen
+from test_hip_llm_ops import IDS, TYPES, U, attention_case, gen, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +127,25 @@ def test_attention_rows_behind_their_lengths_beside_bad_keys_with_more_scores_th
     o, lse = ops.cross_attention(q, k, v, q_lens=q_lens, need_lse=True)
     dq, _, _ = ops.cross_attention_bwd(q, k, v, o, lse, do, q_lens=q_lens)
     assert float(dq[0, 8100:].abs().max()) == 0.0 and bool(torch.isnan(dq[0, :8100]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("Nq,Nk", [(2, 1), (2, 100), (2, 5000), (70, 1), (70, 100), (70, 5000)])
+def test_attention_of_a_nan_row(dtype, Nq, Nk):
+    """a NaN query row looks at keys: its output and its log sum exp are NaN, not those of a row without a key; and so where every key is NaN"""
+    from ogmm_amd import ops
+    q, k, v, do = attention_case(1, Nq, Nk, 2, 1, 32, dtype, 8)
+    good, lse_good = ops.cross_attention(q, k, v, need_lse=True)
+    q2 = q.clone()
+    q2[0, 1, 0] = math.nan
+    o, lse = ops.cross_attention(q2, k, v, need_lse=True)
+    assert bool(torch.isnan(o[0, 1, 0]).all()) and math.isnan(float(lse[0, 0, 1]))
+    others = torch.ones(1, Nq, 2, dtype=torch.bool, device="cuda")
+    others[0, 1, 0] = False
+    # (a NaN makes its wave look for the other rows' maxima anew: their weights stand at another power, one more rounding each)
+    assert float((o[others].double() - good[others].double()).norm()) <= 4 * (half_step(dtype) + 64 * U) * float(good[others].double().norm())
+    assert bool(((lse - lse_good)[others.transpose(1, 2)].abs() <= 2 * (Nk + 64) * U + 8 * U * lse_good[others.transpose(1, 2)].abs()).all())
+    dq, _, _ = ops.cross_attention_bwd(q2, k, v, o, lse, do)
+    assert bool(torch.isnan(dq[0, 1, 0]).all()) and bool(torch.isfinite(dq[others]).all())
+    o, lse = ops.cross_attention(q, k * math.nan, v, need_lse=True)
+    assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
