@@ -74,7 +74,8 @@ class Trainer:
         2^16 with precision "f16x3", 1 with "f32".  If a scaled gradient exceeds 65504 the engine raises its overflow flag:
         the step is skipped and the scale halved.
         max_grad_norm: a limit for the global norm of the (all-reduced, un-scaled) gradients; a larger one is scaled down to it before the optimizer, in the same pass
-        that un-scales (ops.clip_grads_).  step() then also returns "grad_norm", the norm before clipping, a scalar on the device.  None: no norm is formed."""
+        that un-scales (ops.clip_grads_).  step() then also returns "grad_norm", the norm before clipping, a scalar on the device; NaN for a skipped step, whose gradients are
+        dropped.  None: no norm is formed."""
         if max_grad_norm is not None and not max_grad_norm >= 0:
             raise ValueError("max_grad_norm must be None or a number that is not negative, got %r" % (max_grad_norm,))
         self.max_grad_norm = max_grad_norm
@@ -227,8 +228,7 @@ class Trainer:
             allreduce_gradients(self.model, self.dist, self.world)
             if self.max_grad_norm is not None:
                 grads = [p.grad for p in self.model.parameters() if p.grad is not None]
-                if grads:
-                    grad_norm = ops.clip_grads_(grads, self.max_grad_norm, inv_scale=1.0 / self._backward_scale)
+                grad_norm = ops.clip_grads_(grads, self.max_grad_norm, inv_scale=1.0 / self._backward_scale) if grads else torch.zeros((), device=src.device)
             elif self._backward_scale != 1.0:
                 grads = [p.grad for p in self.model.parameters() if p.grad is not None]
                 torch._foreach_mul_(grads, 1.0 / self._backward_scale)          # one multi-tensor launch instead of 150 small ones
@@ -239,8 +239,8 @@ class Trainer:
             r_err = metric.rotation_error(out[0], transform_gt[:, :3, :3]).mean()
             t_err = metric.translation_error(out[1], transform_gt[:, :3, 3].reshape(B, 3)).mean()
         info = {"loss": loss, "skipped": overflowed, "parts": parts, "r_err_deg": r_err, "t_err": t_err, "out": out}
-        if grad_norm is not None:
-            info["grad_norm"] = grad_norm
+        if self.max_grad_norm is not None:
+            info["grad_norm"] = torch.full((), float("nan"), device=src.device) if grad_norm is None else grad_norm
         return info
 
 

@@ -1,6 +1,10 @@
 """CPU: what the entries of cross attention, RMS norm and gradient clipping, and the trainer around them, decide on the host."""
+import math
 import os
 import re
+
+import pytest
+import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -12,3 +16,26 @@ def test_nothing_turns_graph_packet_capture_on():
             if name.endswith((".py", ".sh")):
                 text = open(os.path.join(ROOT, folder, name), encoding="utf-8").read()
                 assert not re.search(r"PACKET_CAPTURE\W{0,8}=\W{0,3}[1-9]", text), os.path.join(folder, name)
+
+
+@pytest.mark.parametrize("hits", [(True, False), (False, True), (True, True), (False, False)])
+@pytest.mark.parametrize("limit", [None, 0.5])
+def test_trainer_returns_a_norm_for_every_step(hits, limit):
+    """with a limit "grad_norm" is there for a skipped step too, as a NaN, and for one that left no gradient, as zero"""
+    from ogmm_amd.trainer import Trainer
+
+    class Steps(Trainer):
+        def _traced(self, src, *_):
+            R, t = torch.eye(3).repeat(src.shape[0], 1, 1), torch.zeros(src.shape[0], 3)
+            return (R, t), torch.ones(()), {}, None, None
+
+        def _overflow_hits(self, fwd, bwd):
+            return hits
+
+    trainer = Steps(torch.nn.Linear(2, 2), max_grad_norm=limit, loss_scale=1.0)
+    for p in trainer.model.parameters():
+        p.requires_grad_(False)
+    info = trainer.step(torch.zeros(2, 3, 4), torch.zeros(2, 3, 4), torch.eye(4).repeat(2, 1, 1), None, None)
+    assert info["skipped"] == any(hits) and ("grad_norm" in info) == (limit is not None)
+    if limit is not None:
+        assert info["grad_norm"].shape == () and (math.isnan(float(info["grad_norm"])) if any(hits) else float(info["grad_norm"]) == 0.0)
