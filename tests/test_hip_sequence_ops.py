@@ -149,3 +149,40 @@ def test_attention_of_a_nan_row(dtype, Nq, Nk):
     assert bool(torch.isnan(dq[0, 1, 0]).all()) and bool(torch.isfinite(dq[others]).all())
     o, lse = ops.cross_attention(q, k * math.nan, v, need_lse=True)
     assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
+
+
+# ---------------------------------------------------------------------------------------------- the trainer's gradients
+@pytest.mark.parametrize("precision,loss_scale", [("f32", None), ("f32", 1024.0), ("f16x3", None)])
+def test_trainer_clips_the_gradients_it_has(precision, loss_scale):
+    """Trainer(max_grad_norm=): tensor by tensor the un-clipped step's gradients, times one factor where they are above the limit, with the loss scale taken out"""
+    from argparse import Namespace
+
+    from ogmm_amd import synth
+    from ogmm_amd.gmmreg import GMMReg
+    from ogmm_amd.trainer import Trainer
+    cfg = Namespace(gnn_k=20, num_heads=4, km_clusters=128, overlap_radius=0.035, n_clusters=16, precision=precision)
+    batch = [b.cuda() for b in synth.make_train_batch(0, 2, 256)]
+    starts = synth.fps_starts_for(0, 2, 256)
+
+    def gradients(limit):
+        model = GMMReg(512, 16, cfg)
+        synth.fill_state_dict(model.state_dict())
+        trainer = Trainer(model.cuda(), welsch_top_k=64, loss_scale=loss_scale, max_grad_norm=limit)
+        info = trainer.step(*batch, fps_starts=starts)
+        assert not info["skipped"]
+        return [None if p.grad is None else p.grad.double() for p in model.parameters()], info
+
+    plain, _ = gradients(None)
+    total = math.sqrt(sum(float(t.square().sum()) for t in plain if t is not None))
+    for limit in (1e9, math.inf, 0.05 * total):
+        got, info = gradients(limit)
+        factor = min(1.0, limit / (total + 1e-6))
+        # (row scatter-adds of the step use atomics: two steps agree to their summation order, 1e-4 of the whole)
+        assert abs(float(info["grad_norm"]) - total) <= 1e-4 * total
+        far = 0.0
+        for a, b in zip(got, plain):
+            assert (a is None) == (b is None)
+            if a is not None:
+                assert bool(a.any()) == bool(b.any())
+                far += float((a - factor * b).square().sum())
+        assert math.sqrt(far) <= 2e-4 * factor * total
