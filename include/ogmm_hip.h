@@ -578,7 +578,7 @@ int ogmm_rms_norm_bwd(const void* dy, int64_t lddy, const void* h, int64_t ldh, 
 /* ---- L3: global norm of n gradient tensors and their clipping: norm = inv_scale sqrt(sum of all squares), c = min(1, max_norm / (norm + 1e-6)), and every gradient times
  * inv_scale c: in place (out = NULL) or into the fp32 tensors out[i].  grads, numel, types, out: HOST arrays of n entries (device pointers, element counts, type codes; read before the
  * call returns); tensors may start at any element.  Squares are summed in fp64 (each four or eight of them in fp32 first, inside its range) in a fixed order.  A norm that is NaN makes the gradients NaN, an infinite one makes them 0 (NaN where they were
- * infinite).  Written memory must not be shared between entries (refused); out[i] may be grads[i] itself where that is fp32.  norm: one fp32 on the device.
+ * infinite), but for max_norm = infinity, which un-scales and no more.  Written memory must not be shared between entries (refused); out[i] may be grads[i] itself where that is fp32.  norm: one fp32 on the device.
  * workspace: ogmm_grad_norm_workspace_bytes(n, numel). */
 int64_t ogmm_grad_norm_workspace_bytes(int n, const int64_t* numel);
 int ogmm_grad_norm(int n, const void* const* grads, const int64_t* numel, const int32_t* types, float inv_scale, float* norm, void* workspace, void* stream);

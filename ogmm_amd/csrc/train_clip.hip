@@ -166,7 +166,7 @@ __global__ __launch_bounds__(THREADS, 8) void grad_clip_kernel(const Table<N, OU
     const double total = norm_of(partial, partials, inv_scale, lds);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(total);
     double c = max_norm / (total + 1e-6);
-    if (c > 1.0) c = 1.0;          // (a NaN stays one: the gradients become NaN as they do in a plain product)
+    if (c > 1.0 || (isinf(max_norm) && isinf(total))) c = 1.0;          // (without a limit nothing is clipped; a NaN stays one: the gradients become NaN as they do in a plain product)
     const float f = static_cast<float>(c * inv_scale);
     if (!OUT && f == 1.0f) return;          // nothing changes
     over_runs(t, n, run, [&](int i, uint32_t off, uint32_t len) {

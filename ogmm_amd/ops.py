@@ -1431,7 +1431,7 @@ def grad_norm(grads, inv_scale=1.0):
 def clip_grads_(grads, max_norm, inv_scale=1.0, out=None):
     """Scales the tensors by inv_scale * min(1, max_norm / (norm + 1e-6)) with norm = grad_norm(grads, inv_scale), in place, or into the fp32 tensors `out` (same shapes; the
     gradients stay as they are).  inv_scale: the inverse of the loss scale that the gradients carry.  max_norm may be infinite (un-scale only).  -> norm, fp32 scalar on the device; no host
-    synchronisation.  A NaN norm makes every gradient NaN.  Tensors that share memory which is written are refused."""
+    synchronisation.  A NaN norm makes every gradient NaN, an infinite one above a finite limit makes them 0 (NaN where they were infinite).  Tensors that share memory which is written are refused."""
     grads, dev, n, ptrs, numel, types = _grad_list(grads)
     outs = None
     if out is not None:

@@ -151,6 +151,23 @@ def test_attention_of_a_nan_row(dtype, Nq, Nk):
     assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
 
 
+# ---------------------------------------------------------------------------------------------- gradients: lists of several runs, tensors in pieces, infinite limits
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_gradients_infinite_norm_without_a_limit(dtype):
+    """max_norm = inf un-scales and does nothing else, also where a gradient is infinite; a NaN still makes all of them NaN"""
+    from ogmm_amd import ops
+    a, b = torch.ones(5000, device="cuda", dtype=dtype), torch.full((33,), 8.0, device="cuda", dtype=dtype)
+    a[17] = math.inf
+    out = [torch.zeros(5000, device="cuda"), torch.zeros(33, device="cuda")]
+    assert math.isinf(float(ops.clip_grads_([a, b], math.inf, inv_scale=0.25, out=out)))
+    assert torch.equal(out[0], a.float() * 0.25) and torch.equal(out[1], b.float() * 0.25)
+    assert math.isinf(float(ops.clip_grads_([a, b], math.inf, inv_scale=0.25)))
+    assert torch.equal(a.float(), out[0]) and torch.equal(b.float(), out[1])
+    a[18] = math.nan
+    assert math.isnan(float(ops.clip_grads_([a, b], math.inf)))
+    assert bool(torch.isnan(a).all()) and bool(torch.isnan(b).all())
+
+
 # ---------------------------------------------------------------------------------------------- the trainer's gradients
 @pytest.mark.parametrize("precision,loss_scale", [("f32", None), ("f32", 1024.0), ("f16x3", None)])
 def test_trainer_clips_the_gradients_it_has(precision, loss_scale):
