@@ -95,6 +95,10 @@ __device__ __forceinline__ float over_row(float v, float* lds, int& slot) {
 
 template <int LANES> constexpr int THREADS = LANES > 256 ? LANES : 256;
 
+// Squares of fp32 or bf16 values leave fp32 from 2^64 on, and below 2^-50 come near the end of its normal numbers: the sum is formed again from the values times a power of two then
+__device__ __forceinline__ bool squares_fit(float ss, float eps) { return ss < INFINITY && (ss > 0x1p-100f || eps > 0x1p-70f); }
+
+
 struct NormArgs {
     const void *x, *r, *w;
     int64_t ldx, ldr, rows;
@@ -140,7 +144,18 @@ __global__ __launch_bounds__(THREADS<LANES>) void rms_norm_kernel(const NormArgs
 #pragma unroll
             for (int k = 0; k < VEC; ++k) ss = fmaf(h[i][k], h[i][k], ss);
         ss = over_row<LANES, false>(ss, lds, slot);
-        const float rstd = 1.0f / sqrtf(ss / D + a.eps);
+        float rstd = 1.0f / sqrtf(ss / D + a.eps);
+        if constexpr (!std::is_same_v<T, _Float16>)
+            if (!squares_fit(ss, a.eps)) {          // (a row's lanes agree)
+                const float k = ss < 1.0f ? 0x1p72f : 0x1p-72f;
+                ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) ss = fmaf(h[i][j] * k, h[i][j] * k, ss);
+                ss = over_row<LANES, false>(ss, lds, slot);
+                rstd = k / sqrtf(ss / D + a.eps * k * k);
+            }
         if constexpr (!Q8) {
             if (a.rstd && here && lane == 0) a.rstd[row] = rstd;
 #pragma unroll

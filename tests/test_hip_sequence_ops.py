@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ogmm_amd          # noqa: F401  (before anything touches the GPU: it switches the runtime's graph packet capture off)
-from test_hip_llm_ops import IDS, TYPES, U, attention_case, gen, half_step
+from test_hip_llm_ops import IDS, TYPES, U, attention_case, close, gen, half_step, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -149,6 +149,41 @@ def test_attention_of_a_nan_row(dtype, Nq, Nk):
     assert bool(torch.isnan(dq[0, 1, 0]).all()) and bool(torch.isfinite(dq[others]).all())
     o, lse = ops.cross_attention(q, k * math.nan, v, need_lse=True)
     assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
+
+
+# ---------------------------------------------------------------------------------------------- RMS norm: rows that loop, magnitudes at the ends
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS.get)
+@pytest.mark.parametrize("D", [5, 96, 500, 2000, 6000, 20000])
+def test_norm_squares_outside_fp32(dtype, D):
+    """rows whose squares, or their sum, leave fp32's range: the norm itself is inside it"""
+    from ogmm_amd import ops
+    g = gen(D)
+    base, w = randn(g, 6, D), (1 + 0.3 * randn(g, D)).to(dtype)
+    dy = randn(g, 6, D, dtype=dtype)
+    sizes = torch.tensor([1e25, 1e-25, 1.0, 3e18, 1e30, 0.0], device="cuda")
+    x = (base * sizes[:, None]).to(dtype)
+    t, n = half_step(dtype), 48 * U
+    for eps in (0.0, 1e-6, 1e-38):
+        H = x.double()
+        RS = 1 / ((H * H).mean(dim=1, keepdim=True) + eps).sqrt()
+        live = [0, 1, 2, 3, 4] if eps == 0.0 else [0, 1, 2, 3, 4, 5]          # (a row of zeros without eps: 0 / 0)
+        Y = H * RS * w.double()
+        y, _, rstd = ops.rms_norm(x, w, eps=eps)
+        close(y[live], Y[live], ((n + t) * Y.abs() + 2.0 ** -140)[live], "y")
+        close(rstd[live], RS[live, 0], n * RS[live, 0], "rstd")
+        assert eps > 0.0 or bool(torch.isnan(y[5]).all())
+        q, s, _ = ops.rms_norm_q8(x, w, eps=eps)
+        S = Y.abs().amax(dim=1, keepdim=True) / 448.0
+        S = torch.where(S < 2.0 ** -126, torch.zeros_like(S), S)
+        close(s[live], S[live], 2 * n * S[live], "scales")
+        Q = q.double() * s.double()
+        close(Q[live], torch.where(S == 0, torch.zeros_like(Y), Y)[live], (torch.maximum(2.0 ** -4 * Y.abs(), 2.0 ** -10 * S) * (1 + 2.0 ** -8) + 4 * n * Y.abs())[live], "q scales")
+        if eps == 0.0:
+            G, XH = dy.double() * w.double(), H * RS
+            DX = RS * (G - XH * (G * XH).mean(dim=1, keepdim=True))
+            size = RS * (G.abs() + XH.abs() * (G * XH).abs().mean(dim=1, keepdim=True))
+            dx, _ = ops.rms_norm_bwd(dy[live], x[live], w, rstd[live])
+            close(dx, DX[live], ((72 * U + 3 * n) * size + t * DX.abs() + 2.0 ** -134)[live], "dx")
 
 
 # ---------------------------------------------------------------------------------------------- gradients: lists of several runs, tensors in pieces, infinite limits
