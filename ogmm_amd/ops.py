@@ -1206,16 +1206,16 @@ def _call_on(dev, name, *args):
         raise _lib.OgmmError("%s failed: %s" % (name, _lib.load().ogmm_last_error().decode(errors="replace")))
 
 
-def _heads(t, name, dtype):
+def _heads(t, name, dtype, group=0):
     """[B, n, heads, d] as the attention kernels take it -> (tensor, its strides of batch, row and head): channels contiguous, address and strides multiples of
-    16 bytes, rows and heads less than 32 MB apart; anything else is copied"""
+    16 bytes, rows and heads less than 32 MB apart, 64 rows and the `group` heads that share a key head within 4 GB; anything else is copied"""
     if t.dim() != 4 or t.dtype != dtype:
         raise _lib.OgmmError("%s must be %s [B, n, heads, d], got %s %s" % (name, dtype, t.dtype, tuple(t.shape)))
     B, N, H, D = t.shape
     b, n, h, one = t.stride()
     b, n, h = b if B > 1 else 0, n if N > 1 else 0, h if H > 1 else 0
     e = t.element_size()
-    if (one != 1 and D > 1) or (b | n | h) * e % 16 or t.data_ptr() % 16 or n * e >= 1 << 25 or h * e >= 1 << 25:
+    if (one != 1 and D > 1) or (b | n | h) * e % 16 or t.data_ptr() % 16 or n * e >= 1 << 25 or h * e >= 1 << 25 or (64 * n + group * h) * e >= 1 << 32:
         t = torch.empty((B, N, H, D), dtype=dtype, device=t.device).copy_(t)
         b, n, h = N * H * D, H * D, D
     return t, b, n, h
@@ -1243,9 +1243,10 @@ class _Xattn:
     def __init__(self, q, k, v, kv_lens, q_lens, key_mask, scale):
         self.dev = _dev("q", q, k=k, v=v, kv_lens=kv_lens, q_lens=q_lens, key_mask=key_mask)
         code = _code(q, "q")
-        self.q, self.k, self.v = _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
-        B, Nq, H, d = q.shape
+        self.k, self.v = _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
         Nk, Hkv = k.shape[1:3]
+        self.q = _heads(q, "q", q.dtype, q.shape[2] // max(Hkv, 1) if q.dim() == 4 else 0)
+        B, Nq, H, d = q.shape
         if k.shape != (B, Nk, Hkv, d) or v.shape != k.shape:
             raise _lib.OgmmError("q %s, k %s and v %s do not fit: [B, Nq, H, d] and twice [B, Nk, Hkv, d]" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
         kv_lens, q_lens = _lens(kv_lens, B, "kv_lens"), _lens(q_lens, B, "q_lens")
@@ -1303,7 +1304,7 @@ def cross_attention_bwd(q, k, v, o, lse, dout, kv_lens=None, q_lens=None, key_ma
     dq = q.new_empty(q.shape)
     dk = k.new_empty(k.shape)
     dv = k.new_empty(k.shape)
-    a.call("ogmm_xattn_bwd", 1, o, rest, lse, _heads(dout, "dout", q.dtype), (dq, dk, dv))
+    a.call("ogmm_xattn_bwd", 1, o, rest, lse, _heads(dout, "dout", q.dtype, H // max(k.shape[2], 1)), (dq, dk, dv))
     return dq, dk, dv
 
 

@@ -151,6 +151,21 @@ def test_attention_of_a_nan_row(dtype, Nq, Nk):
     assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
 
 
+# ---------------------------------------------------------------------------------------------- cross attention: sizes from which other routes are taken
+def test_attention_of_heads_far_apart():
+    """256 heads that share a key head, 16 MB from one to the next: further than the kernels' 32 bits reach, so they are copied"""
+    from ogmm_amd import ops
+    q, k, v, do = attention_case(1, 3, 40, 256, 256, 8, torch.bfloat16, 23)
+    far = torch.empty((1 << 31) + (1 << 23), dtype=torch.bfloat16, device="cuda").as_strided(q.shape, (8, 8, 1 << 23, 1))
+    far.copy_(q)
+    o, lse = ops.cross_attention(q, k, v, need_lse=True)
+    assert torch.equal(ops.cross_attention(far, k, v), o)
+    want = ops.cross_attention_bwd(q, k, v, o, lse, do)
+    assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention_bwd(far, k, v, o, lse, do), want))
+    far.copy_(do)
+    assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention_bwd(q, k, v, o, lse, far), want))
+
+
 # ---------------------------------------------------------------------------------------------- RMS norm: rows that loop, magnitudes at the ends
 @pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS.get)
 @pytest.mark.parametrize("D", [5, 96, 500, 2000, 6000, 20000])

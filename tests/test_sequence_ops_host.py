@@ -39,3 +39,18 @@ def test_trainer_returns_a_norm_for_every_step(hits, limit):
     assert info["skipped"] == any(hits) and ("grad_norm" in info) == (limit is not None)
     if limit is not None:
         assert info["grad_norm"].shape == () and (math.isnan(float(info["grad_norm"])) if any(hits) else float(info["grad_norm"]) == 0.0)
+
+
+def test_heads_that_the_kernels_cannot_reach_are_copied():
+    """the attention entries take 64 rows and the heads that share a key head within 4 GB; rows, heads or addresses beyond what they take become a copy"""
+    from ogmm_amd import ops
+    far = torch.empty((1 << 31) + (1 << 23), dtype=torch.bfloat16)          # (never touched but where the heads lie)
+    for heads, step, group, kept in ((256, 1 << 23, 256, False), (256, 1 << 23, 8, True), (250, 1 << 23, 250, True), (2, 1 << 24, 1, False), (4, 64, 4, True), (4, 60, 4, False)):
+        t = far.as_strided((1, 3, heads, 8), (8, 8, step, 1))
+        if kept:
+            assert ops._heads(t, "q", t.dtype, group)[0] is t
+        else:
+            for i in range(heads):
+                t[:, :, i].fill_(i)
+            x, _, n, h = ops._heads(t, "q", t.dtype, group)
+            assert x.is_contiguous() and (n, h) == (heads * 8, 8) and torch.equal(x, t)
