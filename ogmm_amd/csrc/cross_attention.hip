@@ -27,6 +27,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int WEIGHT_LOG2 = 12;          // the forward's weights are 2^12 at most
 
 struct Args : ogmm_xattn {
     int G, rows;                   // query heads to a key head, query rows to a key head (Nq G)
@@ -100,7 +101,7 @@ struct Tile {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float x[DB];
-                __builtin_memcpy(x, __builtin_assume_aligned(p + (8 * (i / 4) + i % 4) * PITCH, DB == 3 ? 4 : 4 * DB), 4 * DB);
+                __builtin_memcpy(x, __builtin_assume_aligned(p + (8 * (i / 4) + i % 4) * PITCH, 4 * DB), 4 * DB);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) c[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[db], __uint_as_float(y[i / 4][i % 4]), c[db], 0, 0, 0);
             }
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
     }
     const int key_tiles = tile * S::ROWS < q_rows ? (len + KT - 1) / KT : 0, per = (key_tiles + a.splits - 1) / a.splits;
     const int end = min(key_tiles, (split + 1) * per);
-    float m = -INFINITY, l = 0.0f;          // m: of scale S log2(e), the running maximum or up to 8 below it
+    float m = -INFINITY, l = 0.0f;          // m: of scale S log2(e), the running maximum or up to WEIGHT_LOG2 below it
     f32x16 o[DB] = {};
     u32x4 rk[St::PASSES], rv[St::PASSES];
     uint8_t bytes[WORDS];
@@ -371,10 +372,10 @@ __global__ __launch_bounds__(64 * WAVES, (Fwd<T, DP, WAVES, KEY_WAVES>::LDS > 81
 #pragma unroll
             for (int u = 1; u < M::CHUNKS; ++u) mma(s, M::row_chunk(lds_k, key0, u), q[u], T());
             // Weights against the maximum that the sums stand at.  Where it is too low, their sum tells: only then is the tile's maximum sought and the sums brought to it.
-            // A weight up to 2^12 keeps its relative precision in every type; what falls below the type's range is 2^-12 of that again.
+            // A weight up to 2^WEIGHT_LOG2 keeps its relative precision in every type; what falls below the type's range is 2^-WEIGHT_LOG2 of that again.
             f32x16 w;
             float part = weights(w, s, c, m);
-            if (__ballot(!(part <= 4096.0f))) {
+            if (__ballot(!(part <= 1 << WEIGHT_LOG2))) {
                 float top = s[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
@@ -1144,7 +1145,10 @@ extern "C" int ogmm_xattn_fwd(const ogmm_xattn* x, void* stream) {
         return with_width(x->d, [&](auto w) {
             using T = decltype(t);
             constexpr int DP = decltype(w)::value;
-            return rows == 32 ? launch_fwd<T, DP, 4, true>(a, as_stream(stream)) : rows == 128 ? launch_fwd<T, DP, 4, false>(a, as_stream(stream)) : launch_fwd<T, DP, 8, false>(a, as_stream(stream));
+            if (rows == 32) return launch_fwd<T, DP, 4, true>(a, as_stream(stream));
+            if constexpr (sizeof(T) * DP <= 128)          // (tile_rows gives 256 rows to narrow heads alone)
+                if (rows == 256) return launch_fwd<T, DP, 8, false>(a, as_stream(stream));
+            return launch_fwd<T, DP, 4, false>(a, as_stream(stream));
         });
     });
 }
