@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ogmm_amd          # noqa: F401  (before anything touches the GPU: it switches the runtime's graph packet capture off)
-from test_hip_llm_ops import IDS, TYPES, U, attention_case, close, gen, half_step, randn
+from test_hip_llm_ops import IDS, TYPES, U, attention_case, check_attention, close, gen, half_step, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -152,6 +152,56 @@ def test_attention_of_a_nan_row(dtype, Nq, Nk):
 
 
 # ---------------------------------------------------------------------------------------------- cross attention: sizes from which other routes are taken
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 32), (torch.float32, 24), (torch.bfloat16, 64), (torch.bfloat16, 40), (torch.float16, 64), (torch.float16, 16)])
+@pytest.mark.parametrize("G", [1, 4])
+def test_attention_many_rows_of_narrow_heads(dtype, d, G):
+    """65536 rows and more of narrow heads: eight waves share a tile of keys"""
+    B, Nq, Nk, H = 2, 8211, 333, 4
+    q, k, v, do = attention_case(B, Nq, Nk, H, G, d, dtype, 6)
+    kv_lens = torch.tensor([Nk, 190], dtype=torch.int32, device="cuda")
+    q_lens = torch.tensor([8000, Nq], dtype=torch.int32, device="cuda")
+    mask = torch.rand(B, Nk, generator=gen(7), device="cuda") < 0.8
+    check_attention(q, k, v, do, grads=False)
+    check_attention(q, k, v, do, grads=False, kv_lens=kv_lens, q_lens=q_lens, key_mask=mask)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_attention_of_many_batch_entries(dtype):
+    """more than 64 entries of different lengths; and 64 of them, all alike but one"""
+    B, Nq, Nk = 70, 40, 100
+    q, k, v, do = attention_case(B, Nq, Nk, 2, 2, 32, dtype, 14)
+    lens = torch.randint(0, Nk + 1, (B,), generator=gen(15), device="cuda", dtype=torch.int32)
+    check_attention(q, k, v, do, kv_lens=lens)
+    lens = torch.full((64,), 50, dtype=torch.int32, device="cuda")
+    lens[63] = 77
+    check_attention(q[:64], k[:64], v[:64], do[:64], kv_lens=lens)
+
+
+def test_attention_gradient_offsets_past_31_bits():
+    """the gradients of a cache of more than 2^31 elements: those of the last batch entry's keys stand where the keys do, all others are zero"""
+    from ogmm_amd import ops
+    B, Nk, Hkv, d, n = 17, 16384 * 8, 8, 128, 700          # 4.6 GB each for k, v and their gradients
+    k = torch.zeros(B, Nk, Hkv, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    g = gen(2)
+    for t in (k, v):
+        t[-1, -n:] = randn(g, n, Hkv, d, dtype=torch.bfloat16)
+    mask = torch.zeros(B, Nk, dtype=torch.bool, device="cuda")
+    mask[-1, -n:] = True
+    q, do = (randn(g, B, 1, 2 * Hkv, d, dtype=torch.bfloat16) for _ in range(2))
+    o, lse = ops.cross_attention(q, k, v, key_mask=mask, need_lse=True)
+    dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, do, key_mask=mask)
+    short = [t[-1:, -n:].clone() for t in (k, v)]
+    o1, lse1 = ops.cross_attention(q[-1:], *short, need_lse=True)
+    want = ops.cross_attention_bwd(q[-1:], *short, o1, lse1, do[-1:])
+    # (the two calls cut the keys differently: fp32 sums in another order, then one rounding each)
+    for x, y in ((o[-1:], o1), (dq[-1:], want[0]), (dk[-1:, -n:], want[1]), (dv[-1:, -n:], want[2])):
+        assert float((x.double() - y.double()).norm()) <= 2 * half_step(torch.bfloat16) * float(y.double().norm())
+    assert float(dq[:-1].abs().max()) == 0.0
+    for x in (dk, dv):
+        assert not bool(x[-1, :-n].any()) and not any(bool(x[b].any()) for b in range(B - 1))
+
+
 def test_attention_of_heads_far_apart():
     """256 heads that share a key head, 16 MB from one to the next: further than the kernels' 32 bits reach, so they are copied"""
     from ogmm_amd import ops
@@ -167,6 +217,39 @@ def test_attention_of_heads_far_apart():
 
 
 # ---------------------------------------------------------------------------------------------- RMS norm: rows that loop, magnitudes at the ends
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("R,D", [(140_001, 16), (70_003, 50), (20_001, 500), (5001, 2060), (1500, 8200), (1100, 16390)])
+def test_norm_more_rows_than_workgroups(dtype, R, D):
+    """every workgroup takes several rows, forward and backward: the first and the last rows and dw against 64 bits, and every row against a call of its own few"""
+    from ogmm_amd import ops
+    g = gen(R)
+    x, r, dy, dh = (randn(g, R, D, dtype=dtype) for _ in range(4))
+    w = (1 + 0.3 * randn(g, D)).to(dtype)
+    y, h, rstd = ops.rms_norm(x, w, r)
+    q, s, _ = ops.rms_norm_q8(x, w, r, group=128)
+    back = (x, r) if dtype != torch.float32 else (h, None)
+    dx, dw = ops.rms_norm_bwd(dy, back[0], w, rstd, dh, residual=back[1])
+    dw64 = torch.zeros(D, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(dw64)
+    step = 777          # rows of a call: one round of every shape
+    for at in range(0, R, step):
+        i = slice(at, at + step)
+        y1, h1, rstd1 = ops.rms_norm(x[i], w, r[i])
+        assert torch.equal(y[i], y1) and torch.equal(h[i], h1) and torch.equal(rstd[i], rstd1)
+        q1, s1, _ = ops.rms_norm_q8(x[i], w, r[i], group=128)
+        assert torch.equal(q[i].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[i], s1)
+        few = slice(at, at + 100)          # (100 rows: one round of the backward)
+        dx1, _ = ops.rms_norm_bwd(dy[few], back[0][few], w, rstd[few], dh[few], residual=None if back[1] is None else back[1][few])
+        assert torch.equal(dx[few], dx1)
+        H = x[i].double() + r[i].double() if dtype != torch.float32 else h[i].double()
+        terms = dy[i].double() * H / ((H * H).mean(dim=1, keepdim=True) + 1e-6).sqrt()
+        dw64 += terms.sum(dim=0)
+        size += terms.abs().sum(dim=0)
+    # as test_norm_gradient_from_the_summands
+    close(dw, dw64, (64 + R // 64 + 48 + 41) * U * size + half_step(dtype) * dw64.abs() + 2.0 ** -25, "dw")
+    assert torch.equal(ops.rms_norm_bwd(dy, back[0], w, rstd, dh, residual=back[1])[1], dw)
+
+
 @pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS.get)
 @pytest.mark.parametrize("D", [5, 96, 500, 2000, 6000, 20000])
 def test_norm_squares_outside_fp32(dtype, D):
@@ -202,6 +285,28 @@ def test_norm_squares_outside_fp32(dtype, D):
 
 
 # ---------------------------------------------------------------------------------------------- gradients: lists of several runs, tensors in pieces, infinite limits
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("sizes", [[20_000_001, 15_000_003, 7, 9_000_000], [(1 << 30) + 5, 3]], ids=["runs", "pieces"])
+def test_gradients_long_lists(dtype, sizes):
+    """more values than one run a workgroup; a tensor longer than one entry of the kernels' table"""
+    from ogmm_amd import ops
+    g = gen(19)
+    grads = [torch.empty(n, device="cuda", dtype=dtype).normal_(generator=g) for n in sizes]
+    parts = [p for t in grads for p in t.split(1 << 26)]
+    total = math.sqrt(sum(float(p.double().square().sum()) for p in parts))
+    assert abs(float(ops.grad_norm(grads)) - total) <= 2 * U * total
+    out = [torch.full(t.shape, math.nan, device="cuda") for t in grads]
+    f = 3.0 / (total / 4 + 1e-6) / 4
+    assert abs(float(ops.clip_grads_(grads, 3.0, inv_scale=0.25, out=out)) - total / 4) <= 2 * U * total / 4
+    for p, o in zip(parts, [o for t in out for o in t.split(1 << 26)]):
+        close(o, p.double() * f, 4 * U * p.double().abs() * f, "out")
+    before = [p.clone() for p in parts]
+    ops.clip_grads_(grads, 3.0, inv_scale=0.25)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for p, b in zip(parts, before):
+        close(p, b.double() * f, (4 * U + half_step(dtype)) * b.double().abs() * f + tiny, "in place")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 def test_gradients_infinite_norm_without_a_limit(dtype):
     """max_norm = inf un-scales and does nothing else, also where a gradient is infinite; a NaN still makes all of them NaN"""
