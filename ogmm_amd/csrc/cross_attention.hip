@@ -11,6 +11,7 @@
 // One row: the keys' bytes: 16 requests of up to 12288 states, 4 key heads of 128, 56 us and 5 to join the parts, 302 MB at 5.4 TB/s; one token to 1024 states: 9 + 3 us, two launches' latency.
 #include "ogmm_common.h"
 #include <algorithm>
+#include <atomic>
 #include <math.h>
 #include <type_traits>
 
@@ -999,19 +1000,23 @@ Args forward_args(const ogmm_xattn* x, float* ws) {
     return a;
 }
 
-// More than 64 KB of LDS is asked for once a device
+// More than 64 KB of LDS is asked for once a device.  Noted when it has been granted: a thread that comes while another asks, asks too.
+struct Granted { std::atomic<bool> on[64]; };
 template <class K>
-int allow_lds(K kernel, int bytes, PerDeviceOnce& once) {
-    if (bytes > 65536 && once.first() && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+int allow_lds(K kernel, int bytes, Granted& granted) {
+    int device = -1;
+    if (bytes <= 65536 || (hipGetDevice(&device) == hipSuccess && device < 64 && granted.on[device])) return 0;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
         return fail("cross attention: %d bytes of LDS are not available", bytes);
+    if (device >= 0 && device < 64) granted.on[device] = true;
     return 0;
 }
 
 template <class T, int DP, int WAVES, bool KEY_WAVES>
 int launch_fwd(Args a, hipStream_t stream) {
     using S = Fwd<T, DP, WAVES, KEY_WAVES>;
-    static PerDeviceOnce once;
-    if (allow_lds(&xattn_fwd_kernel<T, DP, WAVES, KEY_WAVES>, S::LDS, once)) return 1;
+    static Granted granted;
+    if (allow_lds(&xattn_fwd_kernel<T, DP, WAVES, KEY_WAVES>, S::LDS, granted)) return 1;
     const uint32_t grid = deal(a, a.items, static_cast<int64_t>(a.tiles) * a.splits);
     xattn_fwd_kernel<T, DP, WAVES, KEY_WAVES><<<grid, S::THREADS, S::LDS, stream>>>(a);
     if (a.splits > 1) {
@@ -1065,8 +1070,8 @@ BwdArgs backward_args(const ogmm_xattn* x, float* ws, int64_t* floats) {
 template <class T, int DP>
 int launch_bwd(BwdArgs a, hipStream_t stream) {
     using S = Bwd<T, DP>;
-    static PerDeviceOnce once_q, once_k;
-    if (allow_lds(&xattn_dq_kernel<T, DP>, S::LDS, once_q) || allow_lds(&xattn_dkv_kernel<T, DP>, S::LDS, once_k)) return 1;
+    static Granted granted_q, granted_k;
+    if (allow_lds(&xattn_dq_kernel<T, DP>, S::LDS, granted_q) || allow_lds(&xattn_dkv_kernel<T, DP>, S::LDS, granted_k)) return 1;
     const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
     auto add = [&](const float* part, int parts, int64_t n, void* out) {
         xattn_add_kernel<T><<<static_cast<uint32_t>((n / 4 + 255) / 256), 256, 0, stream>>>(part, parts, n, static_cast<T*>(out));

@@ -216,6 +216,37 @@ def test_attention_of_heads_far_apart():
     assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention_bwd(q, k, v, o, lse, far), want))
 
 
+def test_operators_called_by_threads_at_once():
+    """four threads, each with a stream of its own, begin with the same calls at the same time: forward, gradient, norm and clipping are those of one thread"""
+    import threading
+
+    from ogmm_amd import ops
+    cases = [attention_case(1, 70, 400, 4, 2, 128, t, i) for i, t in enumerate([torch.float32, torch.bfloat16, torch.float16, torch.bfloat16])]
+    got, go = [None] * len(cases), threading.Barrier(len(cases))
+
+    def work(i):
+        q, k, v, do = cases[i]
+        o, lse = ops.cross_attention(q, k, v, need_lse=True)
+        dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, do)
+        y, _, rstd = ops.rms_norm(dq, v[0, 0, 0])
+        return [o, lse, dq, dk, dv, y, rstd, ops.clip_grads_([dk, dv], 0.5)]
+
+    def thread(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            go.wait()
+            got[i] = work(i)
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(len(cases)):
+        assert got[i] is not None and all(torch.equal(a, b) for a, b in zip(got[i], work(i)))
+
+
 # ---------------------------------------------------------------------------------------------- RMS norm: rows that loop, magnitudes at the ends
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 @pytest.mark.parametrize("R,D", [(140_001, 16), (70_003, 50), (20_001, 500), (5001, 2060), (1500, 8200), (1100, 16390)])
