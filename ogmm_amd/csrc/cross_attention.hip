@@ -7,7 +7,8 @@
 //
 // What bounds it, measured: many rows in 16 bits: matrix and vector instructions together (heads of 128: the matrix pipes are busy a third of the time, the exponentials, sums and
 // roundings take as long, and both wait at a tile's barrier): 64 x 1024 rows to 717 keys, 4 heads of 128, fp16 153 us = 630 TFLOP/s; 4 x 4096 to 4096, 16 heads over 4, bf16 724 us = 760;
-// 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16 176 us.  fp32: the fp32 matrix pipes, busy four fifths of the time (120 TFLOP/s of the 154 that a large product reaches).
+// 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16 173 us.  16 x 1024 rows to 717 ragged keys, 4 heads of 128, fp32 197 us = 93 TFLOP/s of the 154 that a
+// large product reaches: the fp32 matrix pipes, busy 79 % of the cycles in which a CU works and 68 % of the time.
 // One row: the keys' bytes: 16 requests of up to 12288 states, 4 key heads of 128, 56 us and 5 to join the parts, 302 MB at 5.4 TB/s; one token to 1024 states: 9 + 3 us, two launches' latency.
 #include "ogmm_common.h"
 #include <algorithm>
@@ -583,7 +584,8 @@ struct Bwd {
     static constexpr int TILE_BYTES = 2 * KT * M::PITCH + 2 * KT * 4, LDS = 2 * TILE_BYTES;
 };
 
-// 4 x 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16: 216 us, the matrix pipes busy 44 % of it beside the exponentials; the scores' bytes are LDS reads of K and V
+// 4 x 4096 rows to 2048 ragged, masked keys, 16 heads of 64 over 4, bf16: 212 us, the matrix pipes busy 44 % of the cycles in which a CU works, 39 % of the time, beside the
+// exponentials; the scores' bytes are LDS reads of K and V
 template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 128 ? 2 : 3)) void xattn_dq_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;
@@ -696,7 +698,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP > 1
     else store_column<T, M>(static_cast<T*>(a.dq) + at, nullptr, dq, f, a.d);
 }
 
-// The same case: 305 us, matrix pipes busy half of it (two waves to a SIMD hold K, V and both sums in registers); fp32, 16 x 1024 rows to 717 keys, heads of 128: 523 us, busy three quarters
+// The same case: 305 us, matrix pipes busy 48 % of the cycles in which a CU works, 37 % of the time (two waves to a SIMD hold K, V and both sums in registers).  fp32, 16 x 1024 rows to 717 ragged
+// keys, heads of 128: 513 us, 72 % and 57 %.  64 x 1024 rows to 717, heads of 128: bf16 369 us, fp16 405, one wave to a SIMD, whose sums move between register files
 template <class T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 128 ? 1 : 2)) void xattn_dkv_kernel(const BwdArgs a) {
     using S = Bwd<T, DP>;

@@ -343,7 +343,8 @@ __global__ __launch_bounds__(THREADS<LANES>, (LANES > 256 ? 4 : 2)) void rms_nor
     }
 }
 
-// dw[c] = sum over the workgroups' shares: 64 columns to a workgroup, sixteen slices of the shares beside each other
+// dw[c] = sum over the workgroups' shares, in fp64: 64 columns to a workgroup, sixteen slices of the shares beside each other.  A share is summed in fp32, over the rows of a lane (131072 rows of 512,
+// fp32: 64 of them) and those side by side in a workgroup, which is most of dw's error: 1.7e-7 of its 2-norm, where fp64 throughout gives 5.8e-8 and its own rounding is 2.5e-8
 template <class W>
 __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restrict__ part, int n, int D, W* __restrict__ dw) {
     __shared__ double lds[16][64];

@@ -1291,7 +1291,8 @@ def cross_attention(q, k, v, kv_lens=None, q_lens=None, key_mask=None, scale=Non
 
 def cross_attention_bwd(q, k, v, o, lse, dout, kv_lens=None, q_lens=None, key_mask=None, scale=None, rest=None):
     """Backward of cross_attention(): (dq, dk, dv) from dout = dL/do and the forward's o and lse (and rest); the scores are formed again.  Gradients of a key head are summed over
-    the query heads that share it; keys that are not admitted and rows behind q_lens get zeros.  Repeated calls agree bit for bit."""
+    the query heads that share it; keys that are not admitted and rows behind q_lens get zeros.  Repeated calls agree bit for bit.
+    float32 keeps its scores' gradients in a workspace of up to 1 GB (2^28 of them; more are formed twice instead)."""
     a = _Xattn(q, k, v, kv_lens, q_lens, key_mask, scale)
     _dev("q", q, o=o, lse=lse, dout=dout, rest=rest)
     B, Nq, _, H, *_, code = a.dims
