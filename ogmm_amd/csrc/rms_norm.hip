@@ -144,20 +144,23 @@ __global__ __launch_bounds__(THREADS<LANES>) void rms_norm_kernel(const NormArgs
 #pragma unroll
             for (int k = 0; k < VEC; ++k) ss = fmaf(h[i][k], h[i][k], ss);
         ss = over_row<LANES, false>(ss, lds, slot);
-        float rstd = 1.0f / sqrtf(ss / D + a.eps);
+        float rstd = 1.0f / sqrtf(ss / D + a.eps), k = 1.0f;          // rstd: of h as it stands here, k times the row
         if constexpr (!std::is_same_v<T, _Float16>)
             if (!squares_fit(ss, a.eps)) {          // (a row's lanes agree)
-                const float k = ss < 1.0f ? 0x1p72f : 0x1p-72f;
+                k = ss < 1.0f ? 0x1p72f : 0x1p-72f;
                 ss = 0.0f;
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) ss = fmaf(h[i][j] * k, h[i][j] * k, ss);
+                    for (int j = 0; j < VEC; ++j) {
+                        h[i][j] *= k;
+                        ss = fmaf(h[i][j], h[i][j], ss);
+                    }
                 ss = over_row<LANES, false>(ss, lds, slot);
-                rstd = k / sqrtf(ss / D + a.eps * k * k);
+                rstd = 1.0f / sqrtf(ss / D + a.eps * k * k);
             }
         if constexpr (!Q8) {
-            if (a.rstd && here && lane == 0) a.rstd[row] = rstd;
+            if (a.rstd && here && lane == 0) a.rstd[row] = rstd * k;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll

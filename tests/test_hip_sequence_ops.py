@@ -315,6 +315,25 @@ def test_norm_squares_outside_fp32(dtype, D):
             close(dx, DX[live], ((72 * U + 3 * n) * size + t * DX.abs() + 2.0 ** -134)[live], "dx")
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS.get)
+@pytest.mark.parametrize("D", [7, 300, 5000])
+def test_norm_values_beside_the_largest_and_smallest(dtype, D):
+    """values so large that times their weight they leave fp32, and rows so small that 1 / sqrt(mean(h^2)) does: y and its 8 bits are of ordinary size"""
+    from ogmm_amd import ops
+    g = gen(D)
+    w = torch.full((D,), 3.0, device="cuda").to(dtype)
+    x = torch.stack([s * (0.5 + 0.5 * torch.rand(D, generator=g, device="cuda")) for s in (3e38, 2.0 ** -130, -2e38)]).to(dtype)
+    H = x.double()
+    Y = H / (H * H).mean(dim=1, keepdim=True).sqrt() * 3.0
+    t, n = half_step(dtype), 48 * U
+    y, _, rstd = ops.rms_norm(x, w, eps=0.0)
+    close(y, Y, (n + t) * Y.abs(), "y")
+    q, s, _ = ops.rms_norm_q8(x, w, eps=0.0)
+    S = Y.abs().amax(dim=1, keepdim=True) / 448.0
+    close(s, S, 2 * n * S, "scales")
+    close(q.double() * s.double(), Y, 2.0 ** -4 * (1 + 2.0 ** -8) * Y.abs() + 4 * n * Y.abs(), "q scales")
+
+
 # ---------------------------------------------------------------------------------------------- gradients: lists of several runs, tensors in pieces, infinite limits
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 @pytest.mark.parametrize("sizes", [[20_000_001, 15_000_003, 7, 9_000_000], [(1 << 30) + 5, 3]], ids=["runs", "pieces"])
